@@ -15,6 +15,8 @@ LIB_PATH = os.environ.get("FLUX_CUDA_LIBRARY") or os.path.join(_HERE, "libflux_c
 
 EPI_STORE_BF16, EPI_STORE_F32, EPI_GATED_RES_F32, EPI_SWIGLU_BF16, EPI_STORE_F32_T = range(5)
 EPI_X_F16, EPI_OUT_F16 = 0x100, 0x200  # or-ed into the epilogue: f16 activations in / out
+F32, F16, BF16 = range(3)  # element types of the calls that take one
+NVFP4, MXFP4 = 16, 32  # formats of a 4-bit matrix: columns per block factor
 
 _lib = None
 
@@ -126,6 +128,19 @@ def _declare(L):
     L.flux_cuda_qwen3_forward_device.restype = c_int
     L.flux_cuda_qwen3_forward_device.argtypes = [c_void_p, ctypes.POINTER(c_int), ctypes.POINTER(c_int), c_int,
                                                  ctypes.POINTER(c_void_p)]
+    L.flux_cuda_fp4_code_bytes.restype = c_ll
+    L.flux_cuda_fp4_code_bytes.argtypes = [c_int, c_int]
+    L.flux_cuda_fp4_scale_bytes.restype = c_ll
+    L.flux_cuda_fp4_scale_bytes.argtypes = [c_int, c_int, c_int]
+    fp4 = ctypes.POINTER(Fp4)
+    L.flux_cuda_fp4_quantize.restype = c_int
+    L.flux_cuda_fp4_quantize.argtypes = [c_void_p, c_void_p, c_int, c_ll, fp4]
+    L.flux_cuda_fp4_dequantize.restype = c_int
+    L.flux_cuda_fp4_dequantize.argtypes = [c_void_p, fp4, c_void_p, c_int, c_ll]
+    L.flux_cuda_gemm_fp4.restype = c_int
+    L.flux_cuda_gemm_fp4.argtypes = [c_void_p, fp4, fp4, c_void_p, c_int, c_ll, c_void_p, c_void_p, c_ll]
+    L.flux_cuda_gemv_fp4.restype = c_int
+    L.flux_cuda_gemv_fp4.argtypes = [c_void_p, c_void_p, c_int, c_ll, c_int, fp4, c_void_p, c_int, c_ll]
     L.flux_cuda_patchify.restype = c_int
     L.flux_cuda_patchify.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int]
     L.flux_cuda_unpatchify.restype = c_int
@@ -234,6 +249,13 @@ class CQwenDims(ctypes.Structure):  # flux_cuda_qwen3_dims
         ("rope_theta", ctypes.c_float), ("out_layers", ctypes.c_int * 3)]
 
 
+class Fp4(ctypes.Structure):
+    """flux_cuda_fp4: a 4-bit matrix in device memory the caller owns. Fp4(codes_ptr, scales_ptr, rows, cols, format,
+    scale); fp4_bytes gives the sizes of the two buffers."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("rows", ctypes.c_int), ("cols", ctypes.c_int),
+                ("format", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
 class CRef(ctypes.Structure):  # flux_cuda_ref
     _fields_ = [("latent", ctypes.POINTER(ctypes.c_float)), ("h", ctypes.c_int), ("w", ctypes.c_int),
                 ("t_offset", ctypes.c_int)]
@@ -336,6 +358,18 @@ class Context:
         check(lib().flux_cuda_group_norm_noalloc(self.handle, x_ptr, int(in16), out_ptr, n_img, pixels, C, gamma_ptr,
                                                  beta_ptr, eps, int(swish), int(f16)))
 
+    def fp4_quantize(self, x_ptr, dtype, ldx, q):
+        check(lib().flux_cuda_fp4_quantize(self.handle, x_ptr, dtype, ldx, q))
+
+    def fp4_dequantize(self, q, out_ptr, dtype, ld):
+        check(lib().flux_cuda_fp4_dequantize(self.handle, q, out_ptr, dtype, ld))
+
+    def gemm_fp4(self, x, w, out_ptr, dtype, ld_out, gate_ptr=None, residual_ptr=None, ld_residual=0):
+        check(lib().flux_cuda_gemm_fp4(self.handle, x, w, out_ptr, dtype, ld_out, gate_ptr, residual_ptr, ld_residual))
+
+    def gemv_fp4(self, x_ptr, x_dtype, ldx, rows, w, out_ptr, dtype, ld_out):
+        check(lib().flux_cuda_gemv_fp4(self.handle, x_ptr, x_dtype, ldx, rows, w, out_ptr, dtype, ld_out))
+
     def patchify(self, out_ptr, in_ptr, batch, channels, H, W, patch):
         check(lib().flux_cuda_patchify(self.handle, out_ptr, in_ptr, batch, channels, H, W, patch))
 
@@ -348,6 +382,14 @@ class Context:
 
 
 # ------------------------------------------------------------------------------------------------ host helpers
+def fp4_bytes(rows, cols, format):
+    """Bytes of the codes and of the scales of a 4-bit matrix."""
+    a, b = lib().flux_cuda_fp4_code_bytes(rows, cols), lib().flux_cuda_fp4_scale_bytes(rows, cols, format)
+    if a < 0 or b < 0:
+        raise FluxCudaError("fp4_bytes: bad rows, cols or format")
+    return a, b
+
+
 def _np():
     import numpy as np
     return np

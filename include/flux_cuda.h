@@ -452,6 +452,59 @@ int flux_cuda_group_norm_noalloc(flux_cuda_ctx *ctx, const void *x, int in16, vo
 int flux_cuda_qk_norm_rope(flux_cuda_ctx *ctx, void *qkv, long long ld, int q_col, int k_col, int seq, int batch,
                            int heads, const float *wq, const float *wk, const float *cos_t, const float *sin_t);
 
+/* ------------------------------------------------------------------------------------------------
+ * 4-bit matrices: the linears of the model with operands of 4 bits (no counterpart in the reference, which computes in
+ * f32). A value is code * block factor * scale: the code e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), one factor per
+ * row and block of columns, one scale for the whole matrix. DEVICE pointers, asynchronous on the context's stream,
+ * capturable (no allocation, no synchronisation); the calls run on the context's device, whichever one is current.
+ *
+ * codes:  row r is 16 * ceil(cols / 32) bytes, the even column of a pair in the low half of its byte; columns past the
+ *         end hold code 0.
+ * scales: one byte per row r and block b, in tiles of 128 rows x 4 blocks of 512 bytes, tile (r / 128, b / 4) at
+ *         ((r / 128) * ceil(blocks / 4) + b / 4) * 512, byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of it (the order
+ *         the tensor cores take); rows and blocks past the end hold 0.
+ * flux_cuda_fp4_quantize writes both, padding included; matrices from elsewhere must keep to it. Both 16-byte aligned;
+ * rows [128 i, ...) of a matrix are a matrix of their own (codes + 128 i * row bytes, scales + i * ceil(blocks / 4) * 512).
+ * ---------------------------------------------------------------------------------------------- */
+#define FLUX_CUDA_NVFP4 16 /* blocks of 16 columns, factor e4m3 (at most 448; 0x7F is NaN) */
+#define FLUX_CUDA_MXFP4 32 /* blocks of 32 columns, factor 2^(byte - 127) (0xFF is NaN) */
+
+typedef struct flux_cuda_fp4 {
+  void *codes, *scales; /* flux_cuda_fp4_code_bytes / _scale_bytes of device memory */
+  int rows, cols;
+  int format;  /* FLUX_CUDA_NVFP4 or FLUX_CUDA_MXFP4 */
+  float scale; /* 1 unless the block factors' range does not fit the values */
+} flux_cuda_fp4;
+
+long long flux_cuda_fp4_code_bytes(int rows, int cols);               /* -1 for a bad argument */
+long long flux_cuda_fp4_scale_bytes(int rows, int cols, int format);
+
+/*
+ * x [rows, cols] (dtype FLUX_CUDA_F32 / F16 / BF16, row pitch ldx elements) -> q's codes and scales. q->scale is an
+ * input: a power of two (2^-100 .. 2^100) that x is divided by first, exactly. With a the largest magnitude of a block
+ * then: NVFP4 factor a / 6 rounded to e4m3 (nearest even, at most 448), MXFP4 factor 2^(floor(log2 a) - 2) (at least
+ * 2^-127); codes x / factor rounded to nearest even, at most +-6. Both are roundings of the exact quotients. A factor
+ * of 0 leaves codes of magnitude 0. A block that holds an infinity or a NaN becomes NaN as a whole.
+ */
+int flux_cuda_fp4_quantize(flux_cuda_ctx *ctx, const void *x, int dtype, long long ldx, const flux_cuda_fp4 *q);
+/* The values back: out [rows, cols] (row pitch ld elements), rounded once; f16 saturates (and is counted). */
+int flux_cuda_fp4_dequantize(flux_cuda_ctx *ctx, const flux_cuda_fp4 *q, void *out, int dtype, long long ld);
+/*
+ * out[m, n] = residual[m, n] + gate[n] * sum_k x[m, k] w[n, k] on the block-scaled tensor-core path: the 4-bit form of
+ * flux_cuda_gemm_bf16's STORE and GATED_RES epilogues. x [M, K], w [N, K] of one format; any M, N >= 0, K >= 1. out of
+ * `dtype` with row pitch ld_out; f32 sums, rounded once (f16 saturates and is counted). gate f32 [N] or NULL (1);
+ * residual f32 [M, N] with row pitch ld_residual, or NULL (0); it may be `out` itself in f32 with the same pitch,
+ * otherwise no output may overlap an input. A NaN factor makes the products of its row or column NaN.
+ */
+int flux_cuda_gemm_fp4(flux_cuda_ctx *ctx, const flux_cuda_fp4 *x, const flux_cuda_fp4 *w, void *out, int dtype,
+                       long long ld_out, const float *gate, const float *residual, long long ld_residual);
+/*
+ * The same product for 0 .. 16 rows of x that stay as they are (x_dtype, row pitch ldx): out[m, n] = sum_k x[m, k]
+ * w[n, k], f32 sums. For single tokens and modulation vectors, where reading the weights is the whole cost.
+ */
+int flux_cuda_gemv_fp4(flux_cuda_ctx *ctx, const void *x, int x_dtype, long long ldx, int rows, const flux_cuda_fp4 *w,
+                       void *out, int dtype, long long ld_out);
+
 /*
  * flux_patchify / flux_unpatchify (flux_kernels.c:1038-1094), device pointers, f32: p x p space-to-depth between
  * VAE latents [B, C, H, W] and DiT latents [B, C p p, H/p, W/p] (new channel = c p p + pi p + pj). Arguments as in
