@@ -42,6 +42,9 @@ int fp4_gemm_init();  // opts the product kernels into large shared memory
 
 static constexpr int FP4_GEMV_MAX_ROWS = 16;
 
+template <int DT>
+constexpr int FP4_SIZE = DT == FLUX_CUDA_F32 ? 4 : 2;
+
 // One f32 value as an output element; f16 saturates (the caller counts through `mx`).
 template <int DT>
 __device__ __forceinline__ void fp4_store(void *out, long long i, float v, float &mx) {

@@ -29,7 +29,7 @@ struct alignas(64) Fp4GemmParams {
   CUtensorMap tm_w, tm_x;    // codes as bytes [rows, pitch], boxes of 128 bytes, 128-byte swizzle
   CUtensorMap tm_ws, tm_xs;  // factor tiles as u32 [row tiles, chunks, 128]
   int M, N, slices;          // k-slices of 256 codes
-  int tiles_m;
+  int tiles_m, tiles;
   int splits;                // CTAs of a cluster that share one output tile, each with its part of the k-slices
   float alpha;
   void *out;
@@ -47,33 +47,35 @@ __host__ __device__ constexpr uint32_t fp4_idesc(int M, int N, int block, uint32
          (static_cast<uint32_t>(M >> 7) << 27) | (id << 29);
 }
 
-// D[tmem] (+)= A[smem] * B[smem] with block factors in TMEM; 64 codes of K. Issued by ONE thread.
-template <int BLOCK>
+// D[tmem] (+)= A[smem] * B[smem] with block factors in TMEM; 64 codes of K. Issued by ONE thread; PAIR: for both CTAs of a
+// pair (M = 256, each CTA holding 128 rows of A and half of the rows of B).
+template <int BLOCK, bool PAIR>
 __device__ __forceinline__ void fp4_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                         uint32_t accumulate) {
-  if (BLOCK == 16)
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-        "}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-        "}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
+#define FX_MMA(GROUP, KIND)                                                                              \
+  asm volatile(                                                                                          \
+      "{\n\t"                                                                                            \
+      ".reg .pred p;\n\t"                                                                                \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                        \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t"             \
+      "}\n" ::"r"(d),                                                                                    \
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                                      \
+      : "memory")
+  if (BLOCK == 16) {
+    if (PAIR) FX_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    else FX_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  } else {
+    if (PAIR) FX_MMA("2", "mxf4.block_scale.scale_vec::2X");
+    else FX_MMA("1", "mxf4.block_scale.scale_vec::2X");
+  }
+#undef FX_MMA
 }
 
 // One 512-byte factor tile from shared memory to four TMEM columns, repeated in the four lane groups.
+template <bool PAIR>
 __device__ __forceinline__ void fp4_copy_factors(uint32_t taddr, uint64_t sdesc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+  if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
 }
 // Shared-memory descriptor of a factor tile: no swizzle, groups of 8 rows x 16 bytes at a stride of 128 bytes.
 __device__ __forceinline__ uint64_t fp4_factor_desc(uint32_t smem_addr) {
@@ -85,10 +87,50 @@ __device__ __forceinline__ uint64_t fp4_factor_desc(uint32_t smem_addr) {
   return d;
 }
 
+// tma_load_2d_pair for three dimensions: into this CTA's shared memory, bytes counted on a barrier of the pair's leader.
+__device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const CUtensorMap *m, uint32_t bar_cluster_addr, int x,
+                                                 int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
+}
+
+// Epilogue of W output rows of this thread's column n, starting at `out` (and `res`): the address runs along a 64-bit
+// chain of adds, the residual is fetched for all rows before the first store, and whole blocks carry no predicates - one
+// warp per scheduler has nothing to hide a branch or a multiply behind (checked and addressed row by row the stores cost
+// 150 cycles each).
+template <int DT, int W>
+__device__ __forceinline__ void fp4_emit(const uint32_t (&r)[W], int rows, uint8_t *out, long long pitch, const uint8_t *res,
+                                         long long res_pitch, float alpha, float g, float &mx) {
+  float v[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) v[j] = g * (alpha * __uint_as_float(r[j]));
+  if (rows >= W) {
+    if (res) {
+      float a[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j, res += res_pitch) a[j] = *reinterpret_cast<const float *>(res);
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] += a[j];
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j, out += pitch) fp4_store<DT>(out, 0, v[j], mx);
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      if (j < rows) fp4_store<DT>(out, 0, res ? v[j] + *reinterpret_cast<const float *>(res) : v[j], mx);
+      out += pitch;
+      if (res) res += res_pitch;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -183,14 +225,14 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
       if (leader) {
 #pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c) {
-          fp4_copy_factors(sfa + 4 * c, fp4_factor_desc(ss + 512 * c));
-          fp4_copy_factors(sfb + 4 * c, fp4_factor_desc(ss + C::S_BYTES + 512 * c));
+          fp4_copy_factors<false>(sfa + 4 * c, fp4_factor_desc(ss + 512 * c));
+          fp4_copy_factors<false>(sfb + 4 * c, fp4_factor_desc(ss + C::S_BYTES + 512 * c));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int c = BLOCK == 16 ? k : k >> 1;
           const uint32_t id = BLOCK == 16 ? 0 : (k & 1) * 2;
-          fp4_mma<BLOCK>(tmem, wd + 2 * k, xd + 2 * k, fp4_idesc(F_BN, BM, BLOCK, id), sfa + 4 * c, sfb + 4 * c,
+          fp4_mma<BLOCK, false>(tmem, wd + 2 * k, xd + 2 * k, fp4_idesc(F_BN, BM, BLOCK, id), sfa + 4 * c, sfb + 4 * c,
                          (i | k) ? 1u : 0u);
         }
         tc_commit(&empty[s]);
@@ -207,11 +249,9 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
     const int live = P.M - m0 < BM ? P.M - m0 : BM;
     const float g = P.gate && n < P.N ? P.gate[n] : 1.0f;
     float mx = 0.f;
-    auto emit = [&](int m, float acc) {
-      float v = g * (P.alpha * acc);
-      if (P.residual) v += P.residual[static_cast<long long>(m) * P.ld_res + n];
-      fp4_store<DT>(P.out, static_cast<long long>(m) * P.ld + n, v, mx);
-    };
+    const long long pitch = P.ld * FP4_SIZE<DT>, res_pitch = P.ld_res * 4;
+    uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * FP4_SIZE<DT>;
+    const uint8_t *res = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + n * 4LL : nullptr;
     constexpr int STEP = BM < 32 ? 16 : 32;
     float *part = reinterpret_cast<float *>(smem);  // every MMA has read its operands by now
     if (ok) {
@@ -226,9 +266,7 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
 #pragma unroll
           for (int j = 0; j < STEP; ++j) part[(c + j) * F_BN + nl] = __uint_as_float(r[j]);
         } else if (n < P.N) {
-#pragma unroll
-          for (int j = 0; j < STEP; ++j)
-            if (c + j < live) emit(m0 + c + j, __uint_as_float(r[j]));
+          fp4_emit<DT, STEP>(r, live - c, out + c * pitch, pitch, res ? res + c * res_pitch : res, res_pitch, P.alpha, g, mx);
         }
       }
     }
@@ -241,7 +279,8 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
         for (int m = rank; m < live; m += P.splits) {
           float acc = 0.f;
           for (int s = 0; s < P.splits; ++s) acc += ld_cluster_f32(map_to_cta(mine + m * F_BN * 4, s));
-          emit(m0 + m, acc);
+          const uint32_t bits[1] = {__float_as_uint(acc)};
+          fp4_emit<DT, 1>(bits, 1, out + m * pitch, pitch, res ? res + m * res_pitch : res, res_pitch, P.alpha, g, mx);
         }
       }
     }
@@ -264,6 +303,196 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
   }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Large products: a pair of CTAs on neighbouring SMs owns a 256 (n) x 256 (m) tile. Each CTA stages its own 128 rows of w
+// and half (128) of the rows of x, so a k-slice costs an SM 38 KB of L2 traffic for 512 tensor cycles, which the L2 can
+// just deliver (a 128 x 256 tile per CTA would need 54 KB). The factors of x are needed in full by both CTAs.
+//
+// TMEM holds 512 columns: two accumulators of 256 and 48 columns of factors do not fit, so the second accumulator starts
+// at column 208 and shares 48 columns with the first. The epilogue takes those columns first and releases the accumulator
+// to the next tile's products as soon as it has them in registers; by then the tile before last has long been drained.
+// ------------------------------------------------------------------------------------------------
+template <int BLOCK>
+struct F2Cfg {
+  static constexpr int CHUNKS = 256 / (4 * BLOCK);
+  static constexpr int X_BYTES = 128 * F_KB;
+  static constexpr int S_BYTES = CHUNKS * 512;
+  static constexpr int STAGE_BYTES = F_W_BYTES + X_BYTES + 3 * S_BYTES;
+  static constexpr int STAGES = BLOCK == 16 ? 5 : 6;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
+  static constexpr int SFA = 464, SFB = SFA + 4 * CHUNKS;  // TMEM columns of the factors
+  static constexpr int ACC1 = 208, SHARED = 48;
+  static_assert(STAGE_BYTES % 1024 == 0 && SMEM <= 232448, "stages are aligned and fit");
+  static_assert(SFB + 8 * CHUNKS <= 512 && ACC1 + 256 <= SFA && ACC1 + SHARED == 256, "TMEM columns");
+};
+
+template <int BLOCK, int DT>
+__global__ void __launch_bounds__(F_THREADS, 1) gemm2_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
+  using C = F2Cfg<BLOCK>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE_BYTES);  // used in the leader only
+  uint64_t *empty = full + C::STAGES;                                                // both CTAs
+  uint64_t *tfull = empty + C::STAGES;                                               // both CTAs
+  uint64_t *drained = tfull + 2;  // leader only, 8 arrivals: the shared columns of a tile are in registers
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&tfull[0], 1);
+    mbar_init(&tfull[1], 1);
+    mbar_init(drained, 8);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+  auto fail = [&](int code) {
+    *abort_flag = 1;
+    atomicCAS(P.err, 0, code);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < P.tiles; tile += num_pairs) {
+        const int m0 = (tile % P.tiles_m) * 256, n0 = (tile / P.tiles_m) * 256 + static_cast<int>(rank) * 128;
+        for (int kb = 0; kb < P.slices; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag)) {
+            fail(KERR_WAIT_EMPTY);
+            ok = false;
+            break;
+          }
+          uint8_t *sw = smem + s * C::STAGE_BYTES, *sx = sw + F_W_BYTES, *ss = sx + C::X_BYTES;
+          const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::STAGE_BYTES);  // both CTAs' bytes
+          tma_load_2d_pair(sw, &P.tm_w, bar, kb * F_KB, n0);
+          tma_load_2d_pair(sx, &P.tm_x, bar, kb * F_KB, m0 + static_cast<int>(rank) * 128);
+          tma_load_3d_pair(ss, &P.tm_ws, bar, 0, kb * C::CHUNKS, n0 / 128);
+          tma_load_3d_pair(ss + C::S_BYTES, &P.tm_xs, bar, 0, kb * C::CHUNKS, m0 / 128);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool leader = elect_one();
+      const uint32_t base = smem_u32(smem);
+      uint32_t it = 0, t = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < P.tiles; tile += num_pairs, ++t) {
+        if (t > 0 && !mbar_wait_warp(drained, (t - 1) & 1, abort_flag)) {
+          if (lane == 0) fail(KERR_WAIT_TMEM_EMPTY);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t d = tmem + (t & 1) * C::ACC1;
+        for (int kb = 0; kb < P.slices; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait_warp(&full[s], (it / C::STAGES) & 1, abort_flag)) {
+            if (lane == 0) fail(KERR_WAIT_FULL);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t sw = base + s * C::STAGE_BYTES, sx = sw + F_W_BYTES, ss = sx + C::X_BYTES;
+          const uint64_t wd = make_smem_desc_sw128(sw, 16, 1024), xd = make_smem_desc_sw128(sx, 16, 1024);
+          if (leader) {
+#pragma unroll
+            for (int c = 0; c < C::CHUNKS; ++c) {
+              fp4_copy_factors<true>(tmem + C::SFA + 4 * c, fp4_factor_desc(ss + 512 * c));
+              fp4_copy_factors<true>(tmem + C::SFB + 8 * c, fp4_factor_desc(ss + C::S_BYTES + 512 * c));
+              fp4_copy_factors<true>(tmem + C::SFB + 8 * c + 4, fp4_factor_desc(ss + 2 * C::S_BYTES + 512 * c));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int c = BLOCK == 16 ? k : k >> 1;
+              const uint32_t id = BLOCK == 16 ? 0 : (k & 1) * 2;
+              fp4_mma<BLOCK, true>(d, wd + 2 * k, xd + 2 * k, fp4_idesc(256, 256, BLOCK, id), tmem + C::SFA + 4 * c,
+                                   tmem + C::SFB + 8 * c, (kb | k) ? 1u : 0u);
+            }
+            tc_commit_pair(&empty[s], 3);
+          }
+        }
+        if (ok && leader) tc_commit_pair(&tfull[t & 1], 3);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    float mx = 0.f;
+    uint32_t t = 0;
+    for (int tile = pair; tile < P.tiles; tile += num_pairs, ++t) {
+      const int m0 = (tile % P.tiles_m) * 256, n = (tile / P.tiles_m) * 256 + static_cast<int>(rank) * 128 + q * 32 + lane;
+      if (!mbar_wait_warp(&tfull[t & 1], (t >> 1) & 1, abort_flag)) {
+        if (lane == 0) fail(KERR_WAIT_TMEM_FULL);
+        break;
+      }
+      tc_fence_after_sync();
+      const int live = n < P.N ? (P.M - m0 < 256 ? P.M - m0 : 256) : 0;
+      const float g = P.gate && n < P.N ? P.gate[n] : 1.0f;
+      const uint32_t acc = tmem + (t & 1) * C::ACC1 + (static_cast<uint32_t>(q * 32) << 16);
+      const long long pitch = P.ld * FP4_SIZE<DT>, res_pitch = P.ld_res * 4;
+      uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * FP4_SIZE<DT>;
+      const uint8_t *res = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + n * 4LL : nullptr;
+      auto emit = [&](const auto &r, int c) {
+        fp4_emit<DT>(r, live - c, out + c * pitch, pitch, res ? res + c * res_pitch : res, res_pitch, P.alpha, g, mx);
+      };
+      // the columns the accumulators share come first: the last 48 of the lower one, the first 48 of the upper one
+      const int first = (t & 1) ? 0 : C::ACC1;
+      {
+        uint32_t a[32], b[16];
+        tc_ld_32x32(acc + first, a);
+        tc_ld_32x16(acc + first + 32, b);
+        tc_wait_ld();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(drained), 0));
+        emit(a, first);
+        emit(b, first + 32);
+      }
+      const int rest = (t & 1) ? C::SHARED : 0;
+      for (int c = 0; c < 192; c += 32) {
+        uint32_t r[32];
+        tc_ld_32x32(acc + rest + c, r);
+        tc_wait_ld();
+        emit(r, rest + c);
+      }
+      uint32_t r[16];
+      tc_ld_32x16(acc + rest + 192, r);
+      tc_wait_ld();
+      emit(r, rest + 192);
+    }
+    sat_report(P.err + 1, DT == FLUX_CUDA_F16, mx);
+  }
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other may still read its shared memory or signal its barriers
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- host
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode4 = nullptr;
 
@@ -280,6 +509,19 @@ static cudaError_t opt_in() {
   return e;
 }
 
+template <int BLOCK>
+static cudaError_t opt_in_pair() {
+  cudaError_t e = cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       F2Cfg<BLOCK>::SMEM);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             F2Cfg<BLOCK>::SMEM);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             F2Cfg<BLOCK>::SMEM);
+  return e;
+}
+
 int fp4_gemm_init() {
   if (!g_encode4) {
     void *fn = nullptr;
@@ -290,7 +532,8 @@ int fp4_gemm_init() {
   }
   const bool ok = opt_in<16, 16>() == cudaSuccess && opt_in<16, 32>() == cudaSuccess && opt_in<32, 16>() == cudaSuccess &&
                   opt_in<32, 32>() == cudaSuccess && opt_in<64, 16>() == cudaSuccess && opt_in<64, 32>() == cudaSuccess &&
-                  opt_in<128, 16>() == cudaSuccess && opt_in<128, 32>() == cudaSuccess;
+                  opt_in<128, 16>() == cudaSuccess && opt_in<128, 32>() == cudaSuccess &&
+                  opt_in_pair<16>() == cudaSuccess && opt_in_pair<32>() == cudaSuccess;
   return ok ? 0 : -2;
 }
 
@@ -327,14 +570,27 @@ static cudaError_t launch_one(const Fp4GemmParams &P, unsigned grid, int dtype, 
   return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_BF16>, dim3(grid), dim3(F_THREADS), smem, st, P.splits, P);
 }
 
+template <int BLOCK>
+static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype, cudaStream_t st) {
+  const size_t smem = F2Cfg<BLOCK>::SMEM;
+  if (dtype == FLUX_CUDA_F32)
+    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F32>, dim3(grid), dim3(F_THREADS), smem, st, 2, P);
+  if (dtype == FLUX_CUDA_F16)
+    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F16>, dim3(grid), dim3(F_THREADS), smem, st, 2, P);
+  return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16>, dim3(grid), dim3(F_THREADS), smem, st, 2, P);
+}
+
 int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st) {
   Fp4GemmParams P;
   memset(&P, 0, sizeof(P));
   const int M = a.x.rows, N = a.w.rows, block = a.x.format;
-  const int bm = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  // pairs of CTAs from the size on at which their 256 x 256 tiles occupy half of the SMs
+  const long long pair_tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
+  const bool pair = M > 128 && pair_tiles * 4 >= num_sms;
+  const int bm = pair ? 256 : M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   const uint32_t chunks = 256 / (4 * block);
-  if (map_codes(&P.tm_w, a.w, F_BN) || map_codes(&P.tm_x, a.x, bm) || map_factors(&P.tm_ws, a.w, chunks, 1) ||
-      map_factors(&P.tm_xs, a.x, chunks, 1))
+  if (map_codes(&P.tm_w, a.w, F_BN) || map_codes(&P.tm_x, a.x, pair ? 128 : bm) || map_factors(&P.tm_ws, a.w, chunks, 1) ||
+      map_factors(&P.tm_xs, a.x, chunks, pair ? 2 : 1))
     return -4;
   P.M = M;
   P.N = N;
@@ -342,7 +598,7 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st
   P.tiles_m = (M + bm - 1) / bm;
   const long long tiles = static_cast<long long>(P.tiles_m) * ((N + F_BN - 1) / F_BN);
   P.splits = 1;
-  while (P.splits < 8 && tiles * P.splits * 2 <= 2LL * num_sms && P.splits * 2 <= P.slices) P.splits *= 2;
+  while (!pair && P.splits < 8 && tiles * P.splits * 2 <= 2LL * num_sms && P.splits * 2 <= P.slices) P.splits *= 2;
   P.alpha = a.x.scale * a.w.scale;
   P.out = a.out;
   P.ld = a.ld_out;
@@ -350,6 +606,12 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st
   P.residual = a.residual;
   P.ld_res = a.ld_residual;
   P.err = err;
+  if (pair) {
+    P.tiles = static_cast<int>(pair_tiles);
+    const int pairs = pair_tiles < num_sms / 2 ? P.tiles : num_sms / 2;
+    cudaError_t e = block == 16 ? launch_pair<16>(P, 2 * pairs, a.dtype, st) : launch_pair<32>(P, 2 * pairs, a.dtype, st);
+    return e == cudaSuccess ? 0 : -8;
+  }
   const unsigned grid = static_cast<unsigned>(tiles * P.splits);
   cudaError_t e;
 #define FX_G(BM) e = block == 16 ? launch_one<BM, 16>(P, grid, a.dtype, st) : launch_one<BM, 32>(P, grid, a.dtype, st)

@@ -265,14 +265,17 @@ def _product(fx, ctx, M, N, K, fmt, out, gated=False, pad=0, in_place=False, sca
 @pytest.mark.parametrize("M,N,K", [
     (1, 1, 1), (1, 128, 64), (1, 130, 256), (1, 300, 2560), (2, 127, 31), (7, 129, 1111), (16, 256, 512), (17, 64, 257),
     (33, 128, 300), (64, 384, 1024), (65, 100, 96), (77, 1001, 1111), (128, 128, 256), (129, 257, 640), (200, 640, 1000),
-    (256, 256, 2048), (300, 513, 96)])
+    (256, 256, 2048), (300, 513, 96),
+    # enough tiles for pairs of CTAs: ragged in every direction, one and several tiles per pair, many k-slices
+    (1290, 2300, 70), (700, 3300, 300), (1025, 2049, 1600), (2600, 5200, 64), (150, 9600, 513)])
 def test_product_sizes(fx, ctx, M, N, K, fmt):
     _product(fx, ctx, M, N, K, fmt, "f32")
 
 
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("gated,in_place", [(False, False), (True, False), (True, True)])
-@pytest.mark.parametrize("M,N,K,pad", [(3, 200, 500, 0), (100, 131, 260, 5), (140, 256, 3000, 8), (520, 700, 300, 1)])
+@pytest.mark.parametrize("M,N,K,pad", [(3, 200, 500, 0), (100, 131, 260, 5), (140, 256, 3000, 8), (520, 700, 300, 1), (1300, 2200, 300, 4),
+                                       (1500, 6000, 296, 3)])
 def test_product_outputs(fx, ctx, M, N, K, pad, gated, in_place, out):
     if in_place and out != "f32":
         pytest.skip("a residual in place is f32")
