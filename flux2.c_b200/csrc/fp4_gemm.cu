@@ -23,7 +23,7 @@ namespace fx {
 static constexpr int F_BN = 128;                  // output columns (rows of w) per CTA
 static constexpr int F_KB = 128;                  // bytes of a row per k-slice: 256 codes
 static constexpr int F_W_BYTES = F_BN * F_KB;     // 16 KB
-static constexpr int F_THREADS = 192;
+static constexpr int F_THREADS = 192;             // producer, issuer and four epilogue warps
 
 struct alignas(64) Fp4GemmParams {
   CUtensorMap tm_w, tm_x;    // codes as bytes [rows, pitch], boxes of 128 bytes, 128-byte swizzle
@@ -97,9 +97,12 @@ __device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const CUtensorM
       : "memory");
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -117,18 +120,59 @@ __device__ __forceinline__ void fp4_emit(const uint32_t (&r)[W], int rows, uint8
     if (res) {
       float a[W];
 #pragma unroll
-      for (int j = 0; j < W; ++j, res += res_pitch) a[j] = *reinterpret_cast<const float *>(res);
+      for (int j = 0; j < W; ++j, res += res_pitch) a[j] = __ldcg(reinterpret_cast<const float *>(res));
 #pragma unroll
       for (int j = 0; j < W; ++j) v[j] += a[j];
     }
 #pragma unroll
     for (int j = 0; j < W; ++j, out += pitch) fp4_store<DT>(out, 0, v[j], mx);
-  } else {
+  } else if (rows > 0) {
+    if (res) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      if (j < rows) fp4_store<DT>(out, 0, res ? v[j] + *reinterpret_cast<const float *>(res) : v[j], mx);
-      out += pitch;
-      if (res) res += res_pitch;
+      for (int j = 0; j < W; ++j, res += res_pitch)
+        if (j < rows) v[j] += __ldcg(reinterpret_cast<const float *>(res));
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j, out += pitch)
+      if (j < rows) fp4_store<DT>(out, 0, v[j], mx);
+  }
+}
+
+// The second half of a split tile: rows [m, m_end) of the tile, every fourth one this warp's, four neighbouring columns
+// per lane, the parts of up to SP CTAs added in rank order. R rows' parts (16 loads) are requested before the first is
+// used: a load from another SM takes most of a microsecond.
+template <int DT, int SP, int R>
+__device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m_end, int n, int N, uint8_t *out,
+                                         long long pitch, const uint8_t *res, long long res_pitch, float alpha,
+                                         const float *gate, float &mx) {
+  float g[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) g[i] = gate && n + i < N ? gate[n + i] : 1.0f;
+  for (; m < m_end; m += 4 * R) {
+    float4 v[SP][R];
+#pragma unroll
+    for (int s = 0; s < SP; ++s) {
+      if (s >= splits) break;
+      const uint32_t from = map_to_cta(part, s);
+#pragma unroll
+      for (int j = 0; j < R; ++j) v[s][j] = ld_cluster_f32x4(from + (m + 4 * j < m_end ? m + 4 * j : m) * F_BN * 4);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      float4 a = v[0][j];
+#pragma unroll
+      for (int s = 1; s < SP; ++s)
+        if (s < splits) a.x += v[s][j].x, a.y += v[s][j].y, a.z += v[s][j].z, a.w += v[s][j].w;
+      const int row = m + 4 * j;
+      if (row >= m_end) continue;
+      const float e[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (n + i >= N) continue;
+        float y = g[i] * (alpha * e[i]);
+        if (res) y += __ldcg(reinterpret_cast<const float *>(res + row * res_pitch + i * 4));
+        fp4_store<DT>(out + row * pitch, i, y, mx);
+      }
     }
   }
 }
@@ -144,7 +188,7 @@ struct FCfg {
   static constexpr int S_BYTES = CHUNKS * 512;
   static constexpr int STAGE_BYTES = F_W_BYTES + X_BYTES + 2 * S_BYTES;
   static constexpr int STAGES = BM >= 128 ? 3 : 4;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 256;
   static constexpr int SF_COLS = CHUNKS * 4;
   static constexpr int TMEM_COLS = BM + 2 * SF_COLS <= 64 ? 64 : BM + 2 * SF_COLS <= 128 ? 128 : 256;
   static_assert(STAGE_BYTES % 1024 == 0, "the swizzled operands of every stage start on 1024 bytes");
@@ -153,10 +197,9 @@ struct FCfg {
 };
 
 template <int BM, int BLOCK, int DT>
-__global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
+__global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
   using C = FCfg<BM, BLOCK>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE_BYTES);
   uint64_t *empty = full + C::STAGES;
   uint64_t *tfull = empty + C::STAGES;
@@ -222,6 +265,8 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
       tc_fence_after_sync();
       const uint32_t sw = base + s * C::STAGE_BYTES, sx = sw + F_W_BYTES, ss = sx + C::X_BYTES;
       const uint64_t wd = make_smem_desc_sw128(sw, 16, 1024), xd = make_smem_desc_sw128(sx, 16, 1024);
+      // a 64-row tile may be the upper half of a factor tile's rows: columns 2 and 3 of its four
+      const uint32_t sfx = sfb + (BM == 64 ? (m0 & 64) / 32 : 0);
       if (leader) {
 #pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c) {
@@ -232,7 +277,7 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
         for (int k = 0; k < 4; ++k) {
           const int c = BLOCK == 16 ? k : k >> 1;
           const uint32_t id = BLOCK == 16 ? 0 : (k & 1) * 2;
-          fp4_mma<BLOCK, false>(tmem, wd + 2 * k, xd + 2 * k, fp4_idesc(F_BN, BM, BLOCK, id), sfa + 4 * c, sfb + 4 * c,
+          fp4_mma<BLOCK, false>(tmem, wd + 2 * k, xd + 2 * k, fp4_idesc(F_BN, BM, BLOCK, id), sfa + 4 * c, sfx + 4 * c,
                          (i | k) ? 1u : 0u);
         }
         tc_commit(&empty[s]);
@@ -273,15 +318,15 @@ __global__ void __launch_bounds__(F_THREADS) gemm_fp4_kernel(const __grid_consta
     if (P.splits > 1) {
       __syncwarp();
       cluster_sync_all();
-      // every CTA of the cluster finishes its share of the tile's rows, adding the parts in rank order
-      if (ok && n < P.N) {
-        const uint32_t mine = smem_u32(part) + nl * 4;
-        for (int m = rank; m < live; m += P.splits) {
-          float acc = 0.f;
-          for (int s = 0; s < P.splits; ++s) acc += ld_cluster_f32(map_to_cta(mine + m * F_BN * 4, s));
-          const uint32_t bits[1] = {__float_as_uint(acc)};
-          fp4_emit<DT, 1>(bits, 1, out + m * pitch, pitch, res ? res + m * res_pitch : res, res_pitch, P.alpha, g, mx);
-        }
+      // every CTA of the cluster finishes its share of the tile's rows
+      if (ok) {
+        const int first = live * rank / P.splits + q, end = live * (rank + 1) / P.splits, nj = n0 + lane * 4;
+        const uint32_t mine = smem_u32(part) + lane * 16;
+        uint8_t *o = static_cast<uint8_t *>(P.out) + m0 * pitch + nj * FP4_SIZE<DT>;
+        const uint8_t *r = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + nj * 4LL : nullptr;
+        if (P.splits <= 2) fp4_join<DT, 2, 8>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
+        else if (P.splits <= 4) fp4_join<DT, 4, 4>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
+        else fp4_join<DT, 8, 2>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
       }
     }
     sat_report(P.err + 1, DT == FLUX_CUDA_F16, mx);
@@ -319,7 +364,7 @@ struct F2Cfg {
   static constexpr int S_BYTES = CHUNKS * 512;
   static constexpr int STAGE_BYTES = F_W_BYTES + X_BYTES + 3 * S_BYTES;
   static constexpr int STAGES = BLOCK == 16 ? 5 : 6;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 256;
   static constexpr int SFA = 464, SFB = SFA + 4 * CHUNKS;  // TMEM columns of the factors
   static constexpr int ACC1 = 208, SHARED = 48;
   static_assert(STAGE_BYTES % 1024 == 0 && SMEM <= 232448, "stages are aligned and fit");
@@ -329,8 +374,7 @@ struct F2Cfg {
 template <int BLOCK, int DT>
 __global__ void __launch_bounds__(F_THREADS, 1) gemm2_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
   using C = F2Cfg<BLOCK>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE_BYTES);  // used in the leader only
   uint64_t *empty = full + C::STAGES;                                                // both CTAs
   uint64_t *tfull = empty + C::STAGES;                                               // both CTAs
@@ -454,29 +498,24 @@ __global__ void __launch_bounds__(F_THREADS, 1) gemm2_fp4_kernel(const __grid_co
         fp4_emit<DT>(r, live - c, out + c * pitch, pitch, res ? res + c * res_pitch : res, res_pitch, P.alpha, g, mx);
       };
       // the columns the accumulators share come first: the last 48 of the lower one, the first 48 of the upper one
-      const int first = (t & 1) ? 0 : C::ACC1;
-      {
-        uint32_t a[32], b[16];
-        tc_ld_32x32(acc + first, a);
-        tc_ld_32x16(acc + first + 32, b);
-        tc_wait_ld();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(drained), 0));
-        emit(a, first);
-        emit(b, first + 32);
-      }
-      const int rest = (t & 1) ? C::SHARED : 0;
-      for (int c = 0; c < 192; c += 32) {
-        uint32_t r[32];
-        tc_ld_32x32(acc + rest + c, r);
-        tc_wait_ld();
-        emit(r, rest + c);
-      }
-      uint32_t r[16];
-      tc_ld_32x16(acc + rest + 192, r);
+      const int shared = (t & 1) ? 0 : C::ACC1, rest = (t & 1) ? C::SHARED : 0;
+      uint32_t a[32], b[16];
+      tc_ld_32x32(acc + shared, a);
+      tc_ld_32x16(acc + shared + 32, b);
       tc_wait_ld();
-      emit(r, rest + 192);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(drained), 0));
+      emit(a, shared);
+      emit(b, shared + 32);
+      for (int c = 0; c < 192; c += 32) {
+        tc_ld_32x32(acc + rest + c, a);
+        tc_wait_ld();
+        emit(a, rest + c);
+      }
+      tc_ld_32x16(acc + rest + 192, b);
+      tc_wait_ld();
+      emit(b, rest + 192);
     }
     sat_report(P.err + 1, DT == FLUX_CUDA_F16, mx);
   }
@@ -580,25 +619,61 @@ static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype,
   return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16>, dim3(grid), dim3(F_THREADS), smem, st, 2, P);
 }
 
+// Which kernel, tile height and split a product gets: the least of the times below, in microseconds, whose constants are
+// measured on a B200 (148 SMs) and matter only relative to one another.
+//   One CTA per tile: 2.5 to start and stop, a k-slice 0.33 while the ring's latency bounds it (0.45 with the three stages
+//   of the 128-row tile) and its bytes over 12 TB/s of L2 when many CTAs run (a pitch off the 128-byte lines costs 1.6
+//   times as much), two CTAs per SM and wave; a split adds a cluster launch and the exchange of the partial tile.
+//   Pairs: a k-slice 0.35, an epilogue of 2 that the next tile's products hide.
+// Measured at 1024 x 1024 x 1024: 64 rows 4.8, 128 rows 5.8, pairs 7.0; 512 x 2560 x 9728: 128 rows 20.8 alone, 16.2 split
+// three ways, pairs 19.2; 1 x 2560 x 9728: 16.0 alone, 6.1 split eight ways; 128 x 2560 x 2560: 64 rows 6.8 alone, 7.6 split
+// in two.
+struct Fp4Choice {
+  int bm, splits;  // bm 256: pairs
+};
+static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_sms) {
+  const long long tn = (N + F_BN - 1) / F_BN;
+  Fp4Choice best = {128, 1};
+  double least = 1e30;
+  for (int bm = 16; bm <= 128; bm *= 2) {
+    if (bm < 64 && M > bm) continue;  // a tile starts on half a factor tile at the least
+    const long long tiles = tn * ((M + bm - 1) / bm);
+    for (int s = 1; s <= 8 && s <= slices; ++s) {
+      const long long ctas = tiles * s, slots = 2LL * num_sms;
+      const double active = ctas < slots ? ctas : slots, waves = (ctas + slots - 1) / slots;
+      const double latency = bm == 128 ? 0.45 : 0.33;
+      const double bytes = active * (F_W_BYTES + bm * F_KB + 4096) / 12e6 * (pitch % 128 ? 1.6 : 1.0);
+      const double t = 2.5 + waves * ((slices + s - 1) / s) * (latency > bytes ? latency : bytes) +
+                       (s == 1 ? waves * bm * 0.012 : waves * (1.2 + 0.04 * bm));
+      if (t < least) least = t, best = {bm, s};
+    }
+    if (bm >= M) break;  // a taller tile would only be emptier
+  }
+  if (M > 128) {
+    const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256), pairs = num_sms / 2;
+    const double waves = (tiles + pairs - 1) / pairs, main = slices * 0.35 * (pitch % 128 ? 1.3 : 1.0) + 0.4;
+    if (2.5 + waves * (main > 2.0 ? main : 2.0) + 2.0 < least) best = {256, 1};
+  }
+  return best;
+}
+
 int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st) {
   Fp4GemmParams P;
   memset(&P, 0, sizeof(P));
   const int M = a.x.rows, N = a.w.rows, block = a.x.format;
-  // pairs of CTAs from the size on at which their 256 x 256 tiles occupy half of the SMs
-  const long long pair_tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
-  const bool pair = M > 128 && pair_tiles * 4 >= num_sms;
-  const int bm = pair ? 256 : M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const int slices = static_cast<int>((static_cast<long long>(a.x.cols) + 255) / 256);
+  const Fp4Choice choice = fp4_choose(M, N, slices, fp4_pitch(a.x.cols), num_sms);
+  const int bm = choice.bm;
+  const bool pair = bm == 256;
   const uint32_t chunks = 256 / (4 * block);
   if (map_codes(&P.tm_w, a.w, F_BN) || map_codes(&P.tm_x, a.x, pair ? 128 : bm) || map_factors(&P.tm_ws, a.w, chunks, 1) ||
       map_factors(&P.tm_xs, a.x, chunks, pair ? 2 : 1))
     return -4;
   P.M = M;
   P.N = N;
-  P.slices = static_cast<int>((static_cast<long long>(a.x.cols) + 255) / 256);
+  P.slices = slices;
   P.tiles_m = (M + bm - 1) / bm;
-  const long long tiles = static_cast<long long>(P.tiles_m) * ((N + F_BN - 1) / F_BN);
-  P.splits = 1;
-  while (!pair && P.splits < 8 && tiles * P.splits * 2 <= 2LL * num_sms && P.splits * 2 <= P.slices) P.splits *= 2;
+  P.splits = choice.splits;
   P.alpha = a.x.scale * a.w.scale;
   P.out = a.out;
   P.ld = a.ld_out;
@@ -607,12 +682,13 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st
   P.ld_res = a.ld_residual;
   P.err = err;
   if (pair) {
+    const long long pair_tiles = static_cast<long long>(P.tiles_m) * ((N + 255) / 256);
     P.tiles = static_cast<int>(pair_tiles);
     const int pairs = pair_tiles < num_sms / 2 ? P.tiles : num_sms / 2;
     cudaError_t e = block == 16 ? launch_pair<16>(P, 2 * pairs, a.dtype, st) : launch_pair<32>(P, 2 * pairs, a.dtype, st);
     return e == cudaSuccess ? 0 : -8;
   }
-  const unsigned grid = static_cast<unsigned>(tiles * P.splits);
+  const unsigned grid = static_cast<unsigned>(static_cast<long long>(P.tiles_m) * ((N + F_BN - 1) / F_BN) * P.splits);
   cudaError_t e;
 #define FX_G(BM) e = block == 16 ? launch_one<BM, 16>(P, grid, a.dtype, st) : launch_one<BM, 32>(P, grid, a.dtype, st)
   if (bm == 16) FX_G(16);
