@@ -110,6 +110,7 @@ int flux_cuda_gemm_fp4(flux_cuda_ctx *ctx, const flux_cuda_fp4 *x, const flux_cu
     if (residual == out && (dtype != FLUX_CUDA_F32 || ld_residual != ld_out))
       return refuse(op, "residual may be out itself only in f32 and with the same row pitch");
   }
+  if (ld_out >= (1LL << 30) || (residual && ld_residual >= (1LL << 30))) return refuse(op, "a row pitch is above 2^30 - 1");
   if (fp4_row_tiles(x->rows) * fp4_row_tiles(w->rows) > 0x3FFFFFFF) return refuse(op, "too many output tiles");
   if (!ctx) return refuse(op, "null context");
   if (x->rows == 0 || w->rows == 0) return FLUX_CUDA_OK;

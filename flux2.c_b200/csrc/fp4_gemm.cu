@@ -24,6 +24,7 @@ static constexpr int F_BN = 128;                  // output columns (rows of w) 
 static constexpr int F_KB = 128;                  // bytes of a row per k-slice: 256 codes
 static constexpr int F_W_BYTES = F_BN * F_KB;     // 16 KB
 static constexpr int F_THREADS = 192;             // producer, issuer and four epilogue warps
+static constexpr int F2_THREADS = 320;            // the same with eight epilogue warps
 
 struct alignas(64) Fp4GemmParams {
   CUtensorMap tm_w, tm_x;    // codes as bytes [rows, pitch], boxes of 128 bytes, 128-byte swizzle
@@ -33,9 +34,8 @@ struct alignas(64) Fp4GemmParams {
   int splits;                // CTAs of a cluster that share one output tile, each with its part of the k-slices
   float alpha;
   void *out;
-  long long ld;
   const float *gate, *residual;
-  long long ld_res;
+  uint32_t pitch, res_pitch;  // bytes from row to row of out and residual
   int *err;
 };
 
@@ -97,6 +97,12 @@ __device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const CUtensorM
       : "memory");
 }
 
+// Arrival on a barrier of the pair's leader that orders no memory: what it releases is TMEM whose loads have completed. The
+// releasing form waits for the epilogue's global stores, a thousand cycles in which the tensor pipe stood still.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -106,35 +112,40 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   return v;
 }
 
-// Epilogue of W output rows of this thread's column n, starting at `out` (and `res`): the address runs along a 64-bit
-// chain of adds, the residual is fetched for all rows before the first store, and whole blocks carry no predicates - one
-// warp per scheduler has nothing to hide a branch or a multiply behind (checked and addressed row by row the stores cost
-// 150 cycles each).
-template <int DT, int W>
-__device__ __forceinline__ void fp4_emit(const uint32_t (&r)[W], int rows, uint8_t *out, long long pitch, const uint8_t *res,
-                                         long long res_pitch, float alpha, float g, float &mx) {
-  float v[W];
+// Epilogue of 16 output rows of this thread's column n, starting at `out` (and `res`): a = alpha * gate. Each row's address
+// is one multiply-add of its own (row pitches are 32 bits, checked on the host), the residual is fetched for all rows
+// before the first store, and whole blocks carry no predicates: one warp per scheduler has nothing to hide a chain of
+// 64-bit additions or a branch behind. Checked and addressed row by row a store cost 150 cycles, along a chain 32.
+template <int DT>
+__device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], int rows, uint8_t *out, uint32_t pitch, const uint8_t *res,
+                                         uint32_t res_pitch, float a, float &mx) {
+  float v[16];
+  if (res) {
 #pragma unroll
-  for (int j = 0; j < W; ++j) v[j] = g * (alpha * __uint_as_float(r[j]));
-  if (rows >= W) {
-    if (res) {
-      float a[W];
+    for (int j = 0; j < 16; ++j)
+      v[j] = j < rows ? __ldcg(reinterpret_cast<const float *>(res + static_cast<uint64_t>(res_pitch) * j)) : 0.f;
 #pragma unroll
-      for (int j = 0; j < W; ++j, res += res_pitch) a[j] = __ldcg(reinterpret_cast<const float *>(res));
+    for (int j = 0; j < 16; ++j) v[j] = fmaf(a, __uint_as_float(r[j]), v[j]);
+  } else {
 #pragma unroll
-      for (int j = 0; j < W; ++j) v[j] += a[j];
+    for (int j = 0; j < 16; ++j) v[j] = a * __uint_as_float(r[j]);
+  }
+  if (rows >= 16) {
+    if (DT == FLUX_CUDA_F32) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) *reinterpret_cast<float *>(out + static_cast<uint64_t>(pitch) * j) = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {  // one conversion for two rows
+        const uint32_t w = pack_16x2_t(v[j], v[j + 1], DT == FLUX_CUDA_F16, mx);
+        *reinterpret_cast<uint16_t *>(out + static_cast<uint64_t>(pitch) * j) = static_cast<uint16_t>(w);
+        *reinterpret_cast<uint16_t *>(out + static_cast<uint64_t>(pitch) * (j + 1)) = static_cast<uint16_t>(w >> 16);
+      }
     }
+  } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j, out += pitch) fp4_store<DT>(out, 0, v[j], mx);
-  } else if (rows > 0) {
-    if (res) {
-#pragma unroll
-      for (int j = 0; j < W; ++j, res += res_pitch)
-        if (j < rows) v[j] += __ldcg(reinterpret_cast<const float *>(res));
-    }
-#pragma unroll
-    for (int j = 0; j < W; ++j, out += pitch)
-      if (j < rows) fp4_store<DT>(out, 0, v[j], mx);
+    for (int j = 0; j < 16; ++j)
+      if (j < rows) fp4_store<DT>(out + static_cast<uint64_t>(pitch) * j, 0, v[j], mx);
   }
 }
 
@@ -147,7 +158,7 @@ __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m
                                          const float *gate, float &mx) {
   float g[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) g[i] = gate && n + i < N ? gate[n + i] : 1.0f;
+  for (int i = 0; i < 4; ++i) g[i] = gate && n + i < N ? alpha * gate[n + i] : alpha;
   for (; m < m_end; m += 4 * R) {
     float4 v[SP][R];
 #pragma unroll
@@ -169,8 +180,8 @@ __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (n + i >= N) continue;
-        float y = g[i] * (alpha * e[i]);
-        if (res) y += __ldcg(reinterpret_cast<const float *>(res + row * res_pitch + i * 4));
+        float y = g[i] * e[i];
+        if (res) y = fmaf(g[i], e[i], __ldcg(reinterpret_cast<const float *>(res + row * res_pitch + i * 4)));
         fp4_store<DT>(out + row * pitch, i, y, mx);
       }
     }
@@ -292,26 +303,26 @@ __global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_con
     if (!ok && lane == 0) fail(KERR_WAIT_TMEM_FULL);
     tc_fence_after_sync();
     const int live = P.M - m0 < BM ? P.M - m0 : BM;
-    const float g = P.gate && n < P.N ? P.gate[n] : 1.0f;
+    const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
     float mx = 0.f;
-    const long long pitch = P.ld * FP4_SIZE<DT>, res_pitch = P.ld_res * 4;
+    const long long pitch = P.pitch, res_pitch = P.res_pitch;
     uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * FP4_SIZE<DT>;
     const uint8_t *res = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + n * 4LL : nullptr;
-    constexpr int STEP = BM < 32 ? 16 : 32;
+    constexpr int STEP = 16;
     float *part = reinterpret_cast<float *>(smem);  // every MMA has read its operands by now
     if (ok) {
+#pragma unroll 1  // see the pair kernel
       for (int c = 0; c < BM; c += STEP) {
         if (c >= live) break;
         uint32_t r[STEP];
         const uint32_t at = tmem + c + (static_cast<uint32_t>(q * 32) << 16);
-        if constexpr (STEP == 16) tc_ld_32x16(at, r);
-        else tc_ld_32x32(at, r);
+        tc_ld_32x16(at, r);
         tc_wait_ld();
         if (P.splits > 1) {
 #pragma unroll
           for (int j = 0; j < STEP; ++j) part[(c + j) * F_BN + nl] = __uint_as_float(r[j]);
         } else if (n < P.N) {
-          fp4_emit<DT, STEP>(r, live - c, out + c * pitch, pitch, res ? res + c * res_pitch : res, res_pitch, P.alpha, g, mx);
+          fp4_emit<DT>(r, live - c, out + c * pitch, P.pitch, res ? res + c * res_pitch : res, P.res_pitch, a, mx);
         }
       }
     }
@@ -372,13 +383,13 @@ struct F2Cfg {
 };
 
 template <int BLOCK, int DT>
-__global__ void __launch_bounds__(F_THREADS, 1) gemm2_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
+__global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
   using C = F2Cfg<BLOCK>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE_BYTES);  // used in the leader only
   uint64_t *empty = full + C::STAGES;                                                // both CTAs
   uint64_t *tfull = empty + C::STAGES;                                               // both CTAs
-  uint64_t *drained = tfull + 2;  // leader only, 8 arrivals: the shared columns of a tile are in registers
+  uint64_t *drained = tfull + 2;  // leader only, 16 arrivals: the shared columns of a tile are in registers
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -392,7 +403,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) gemm2_fp4_kernel(const __grid_co
     }
     mbar_init(&tfull[0], 1);
     mbar_init(&tfull[1], 1);
-    mbar_init(drained, 8);
+    mbar_init(drained, 16);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -478,7 +489,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) gemm2_fp4_kernel(const __grid_co
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;
+    const int q = warp & 3, half = warp >= 6;
     float mx = 0.f;
     uint32_t t = 0;
     for (int tile = pair; tile < P.tiles; tile += num_pairs, ++t) {
@@ -489,33 +500,36 @@ __global__ void __launch_bounds__(F_THREADS, 1) gemm2_fp4_kernel(const __grid_co
       }
       tc_fence_after_sync();
       const int live = n < P.N ? (P.M - m0 < 256 ? P.M - m0 : 256) : 0;
-      const float g = P.gate && n < P.N ? P.gate[n] : 1.0f;
+      const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
       const uint32_t acc = tmem + (t & 1) * C::ACC1 + (static_cast<uint32_t>(q * 32) << 16);
-      const long long pitch = P.ld * FP4_SIZE<DT>, res_pitch = P.ld_res * 4;
+      const long long pitch = P.pitch, res_pitch = P.res_pitch;
       uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * FP4_SIZE<DT>;
       const uint8_t *res = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + n * 4LL : nullptr;
-      auto emit = [&](const auto &r, int c) {
-        fp4_emit<DT>(r, live - c, out + c * pitch, pitch, res ? res + c * res_pitch : res, res_pitch, P.alpha, g, mx);
+      // Two warps share a lane group and take every other sixteen columns, in an order that starts with the columns the
+      // accumulators share (the last 48 of the lower one, the first 48 of the upper one): once the first two loads of
+      // each are done the next tile's products may start. Two warps per scheduler, because the epilogue is bound by
+      // instruction latency (8 instructions and 26 cycles per column with one); the loop is not unrolled further, because
+      // 40 KB of straight-line code ran at the speed of instruction fetches and took the issuer's loop out of the cache.
+      const int shared = (t & 1) ? 0 : C::ACC1;
+      uint32_t r0[16], r1[16];
+      auto column = [&](int i) { return (shared + 16 * (2 * i + half)) & 255; };
+      auto finish = [&](const uint32_t (&r)[16], int c) {
+        fp4_emit<DT>(r, live - c, out + c * pitch, P.pitch, res ? res + c * res_pitch : res, P.res_pitch, a, mx);
       };
-      // the columns the accumulators share come first: the last 48 of the lower one, the first 48 of the upper one
-      const int shared = (t & 1) ? 0 : C::ACC1, rest = (t & 1) ? C::SHARED : 0;
-      uint32_t a[32], b[16];
-      tc_ld_32x32(acc + shared, a);
-      tc_ld_32x16(acc + shared + 32, b);
+      tc_ld_32x16(acc + column(0), r0);
+      tc_ld_32x16(acc + column(1), r1);
       tc_wait_ld();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(drained), 0));
-      emit(a, shared);
-      emit(b, shared + 32);
-      for (int c = 0; c < 192; c += 32) {
-        tc_ld_32x32(acc + rest + c, a);
+      if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(drained), 0));
+#pragma unroll 1
+      for (int i = 0; i < 8; i += 2) {
+        finish(r0, column(i));
+        if (i < 6) tc_ld_32x16(acc + column(i + 2), r0);
+        finish(r1, column(i + 1));
+        if (i < 6) tc_ld_32x16(acc + column(i + 3), r1);
         tc_wait_ld();
-        emit(a, rest + c);
       }
-      tc_ld_32x16(acc + rest + 192, b);
-      tc_wait_ld();
-      emit(b, rest + 192);
     }
     sat_report(P.err + 1, DT == FLUX_CUDA_F16, mx);
   }
@@ -613,10 +627,10 @@ template <int BLOCK>
 static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype, cudaStream_t st) {
   const size_t smem = F2Cfg<BLOCK>::SMEM;
   if (dtype == FLUX_CUDA_F32)
-    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F32>, dim3(grid), dim3(F_THREADS), smem, st, 2, P);
+    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F32>, dim3(grid), dim3(F2_THREADS), smem, st, 2, P);
   if (dtype == FLUX_CUDA_F16)
-    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F16>, dim3(grid), dim3(F_THREADS), smem, st, 2, P);
-  return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16>, dim3(grid), dim3(F_THREADS), smem, st, 2, P);
+    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F16>, dim3(grid), dim3(F2_THREADS), smem, st, 2, P);
+  return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16>, dim3(grid), dim3(F2_THREADS), smem, st, 2, P);
 }
 
 // Which kernel, tile height and split a product gets: the least of the times below, in microseconds, whose constants are
@@ -676,10 +690,10 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st
   P.splits = choice.splits;
   P.alpha = a.x.scale * a.w.scale;
   P.out = a.out;
-  P.ld = a.ld_out;
+  P.pitch = static_cast<uint32_t>(a.ld_out * (a.dtype == FLUX_CUDA_F32 ? 4 : 2));
   P.gate = a.gate;
   P.residual = a.residual;
-  P.ld_res = a.ld_residual;
+  P.res_pitch = static_cast<uint32_t>(a.ld_residual * 4);
   P.err = err;
   if (pair) {
     const long long pair_tiles = static_cast<long long>(P.tiles_m) * ((N + 255) / 256);
