@@ -9,14 +9,17 @@
 // bits, so the border b has t = b s with at most seven, and |x - t| >= ulp(x) >= 2^-24 |t| keeps the quotient at least
 // half an ulp away).
 //
-// Bound by memory: every element is read once, 0.56 bytes per element are written. A block of 256 threads owns 128 rows x
-// 256 columns, 16 consecutive columns per thread, so that a thread has a whole block of 16 (half a block of 32) in
-// registers and the factors of a tile leave as whole 512-byte tiles.
+// Bound by memory: every element is read once, 0.56 bytes per element are written. A thread owns 16 consecutive columns of
+// the four rows r, r + 32, r + 64, r + 96 of a 128-row tile: a whole block of 16 (half a block of 32) per row in registers,
+// 128 to 256 bytes of loads in flight per thread, and of the factors exactly what lies in one 16-byte piece of a factor
+// tile, so the four lanes of a chunk put a piece together with shuffles and store it whole. No shared memory, no barrier:
+// rows beyond the last cost one predicate, which keeps a single token at the price of a launch.
 #include "fp4.cuh"
 
 namespace fx {
 
-static constexpr int Q_ROWS = 128, Q_COLS = 256, Q_THREADS = 256;
+static constexpr int Q_COLS = 256;  // columns per block of threads: 16 threads of 16
+static constexpr int Q_THREADS = 128;  // 8 rows r per block of threads, 32 rows of the matrix
 
 template <int DT>
 __device__ __forceinline__ float q_load1(const void *x, long long i) {
@@ -36,30 +39,28 @@ __device__ __forceinline__ void q_expand(uint32_t w, float &lo, float &hi) {
   }
 }
 
-// 16 consecutive elements starting at element i, all in range; ALIGN: bytes the address is a multiple of (16) or 0.
-template <int DT, int ALIGN>
-__device__ __forceinline__ void q_load16(const void *x, long long i, float (&v)[16]) {
-  if (ALIGN == 0) {
+// 16 consecutive elements as 32-bit words, from a 32-byte aligned address.
+template <int DT>
+struct Raw16 {
+  static constexpr int N = DT == FLUX_CUDA_F32 ? 16 : 8;
+  uint32_t w[N];
+};
+template <int DT>
+__device__ __forceinline__ void q_load_raw(const void *x, long long i, Raw16<DT> &raw) {
+  const char *p = reinterpret_cast<const char *>(x) + i * FP4_SIZE<DT>;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = q_load1<DT>(x, i + k);
-  } else if (DT == FLUX_CUDA_F32) {
-    const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(x) + i);
+  for (int k = 0; k < Raw16<DT>::N; k += 8)
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(raw.w[k]), "=r"(raw.w[k + 1]), "=r"(raw.w[k + 2]), "=r"(raw.w[k + 3]), "=r"(raw.w[k + 4]),
+                   "=r"(raw.w[k + 5]), "=r"(raw.w[k + 6]), "=r"(raw.w[k + 7])
+                 : "l"(p + k * 4));
+}
+template <int DT>
+__device__ __forceinline__ void q_expand16(const Raw16<DT> &raw, float (&v)[16]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float4 f = __ldg(p + k);
-      v[4 * k] = f.x, v[4 * k + 1] = f.y, v[4 * k + 2] = f.z, v[4 * k + 3] = f.w;
-    }
-  } else {
-    const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(x) + i);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint4 u = __ldg(p + k);
-      q_expand<DT>(u.x, v[8 * k], v[8 * k + 1]);
-      q_expand<DT>(u.y, v[8 * k + 2], v[8 * k + 3]);
-      q_expand<DT>(u.z, v[8 * k + 4], v[8 * k + 5]);
-      q_expand<DT>(u.w, v[8 * k + 6], v[8 * k + 7]);
-    }
-  }
+  for (int k = 0; k < 16; ++k)
+    if (DT == FLUX_CUDA_F32) v[k] = __uint_as_float(raw.w[k % Raw16<DT>::N]);
+    else if (!(k & 1)) q_expand<DT>(raw.w[k / 2], v[k], v[k + 1]);
 }
 
 // Codes of 16 columns and the factor byte of their block. For blocks of 32 the two threads of a block exchange their
@@ -108,59 +109,66 @@ __device__ __forceinline__ uint32_t q_encode(float (&v)[16], float inv_scale, ui
   return byte;
 }
 
-template <int DT, int BLOCK, int ALIGN>
+// VEC: x and its row pitch are multiples of 32 bytes. Grid: [row tiles][4 groups of 8 rows r][column tiles].
+template <int DT, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) fp4_quantize_kernel(const void *__restrict__ x, long long ldx, int rows,
                                                                  int cols, float inv_scale, uint8_t *__restrict__ codes,
                                                                  long long pitch, uint8_t *__restrict__ scales,
                                                                  long long chunks, int col_tiles) {
-  constexpr int CH = Q_COLS / (4 * BLOCK);  // factor tiles per block of threads
-  __shared__ __align__(16) uint8_t fac[CH * 512];
   pdl_launch_dependents();
-  const long long rt = blockIdx.x / col_tiles;
-  const int ct = blockIdx.x % col_tiles;
-  const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
-  const int here = static_cast<int>(rows - rt * Q_ROWS < Q_ROWS ? rows - rt * Q_ROWS : Q_ROWS);
-  const long long c0 = static_cast<long long>(ct) * Q_COLS + cx * 16;
-  if (threadIdx.x < CH * 32) reinterpret_cast<uint4 *>(fac)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-  __syncthreads();
-#pragma unroll 4
-  for (int it = 0; it < Q_ROWS / 16; ++it) {
-    const int rl = it * 16 + ry;
-    if (it * 16 >= here) break;  // uniform in the block
-    const long long r = rt * Q_ROWS + rl;
+  const int ct = blockIdx.x % col_tiles, rg = blockIdx.x / col_tiles % 4;
+  const long long rt = blockIdx.x / col_tiles / 4;
+  const int cx = threadIdx.x & 15, r32 = rg * 8 + (threadIdx.x >> 4);
+  const long long c0 = static_cast<long long>(ct) * Q_COLS + cx * 16, r0 = rt * 128 + r32;
+  const bool whole = VEC && c0 + 16 <= cols;
+  Raw16<DT> raw[4];
+  if (whole) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (r0 + 32 * q < rows) q_load_raw<DT>(x, (r0 + 32 * q) * ldx + c0, raw[q]);
+  }
+  uint32_t word[4];  // the factors of this lane's chunk of four blocks
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    word[q] = 0;
+    const bool live = r0 + 32 * q < rows;
+    if (!__any_sync(0xffffffffu, live)) continue;
     float v[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k] = 0.f;
-    if (rl < here) {
-      if (c0 + 16 <= cols) {
-        q_load16<DT, ALIGN>(x, r * ldx + c0, v);
+    if (live) {
+      if (whole) {
+        q_expand16<DT>(raw[q], v);
       } else {
+        const long long at = (r0 + 32 * q) * ldx + c0;
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          if (c0 + k < cols) v[k] = q_load1<DT>(x, r * ldx + c0 + k);
+          if (c0 + k < cols) v[k] = q_load1<DT>(x, at + k);
       }
     }
     uint2 cd;
-    const uint32_t byte = q_encode<BLOCK>(v, inv_scale, cd);
-    if (rl < here) {
-      if (c0 / 2 + 8 <= pitch) *reinterpret_cast<uint2 *>(codes + r * pitch + c0 / 2) = cd;
-      const int b = cx * 16 / BLOCK;
-      if (BLOCK == 16 || !(cx & 1))
-        fac[(b >> 2) * 512 + (rl & 31) * 16 + (rl >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(c0 < cols ? byte : 0u);
+    uint32_t byte = q_encode<BLOCK>(v, inv_scale, cd);
+    if (live && c0 / 2 + 8 <= pitch) *reinterpret_cast<uint2 *>(codes + (r0 + 32 * q) * pitch + c0 / 2) = cd;
+    if (c0 >= cols) byte = 0;
+    if (BLOCK == 16) {  // lanes 4 i .. 4 i + 3 hold the four blocks of a chunk
+      byte |= __shfl_xor_sync(0xffffffffu, byte, 1) << 8;
+      byte |= __shfl_xor_sync(0xffffffffu, byte, 2) << 16;
+    } else {  // lanes 8 i, + 2, + 4, + 6
+      byte |= __shfl_xor_sync(0xffffffffu, byte, 2) << 8;
+      byte |= __shfl_xor_sync(0xffffffffu, byte, 4) << 16;
     }
+    word[q] = byte;
   }
-  __syncthreads();
-  const long long chunk = static_cast<long long>(ct) * CH + (threadIdx.x >> 5);
-  if (threadIdx.x < CH * 32 && chunk < chunks)
-    *reinterpret_cast<uint4 *>(scales + (rt * chunks + chunk) * 512 + (threadIdx.x & 31) * 16) =
-        reinterpret_cast<const uint4 *>(fac)[threadIdx.x];
+  const long long chunk = c0 / (4 * BLOCK);
+  if (!(cx & (BLOCK == 16 ? 3 : 7)) && chunk < chunks)
+    *reinterpret_cast<uint4 *>(scales + (rt * chunks + chunk) * 512 + r32 * 16) = make_uint4(word[0], word[1], word[2], word[3]);
 }
 
 int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda_fp4 &q, cudaStream_t st) {
   const int col_tiles = (q.cols + Q_COLS - 1) / Q_COLS;
-  const long long blocks = fp4_row_tiles(q.rows) * col_tiles;
+  const long long blocks = fp4_row_tiles(q.rows) * 4 * col_tiles;
   const int size = dtype == FLUX_CUDA_F32 ? 4 : 2;
-  const bool vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !((ldx * size) & 15);
+  const bool vec = !(reinterpret_cast<uintptr_t>(x) & 31) && !((ldx * size) & 31);
   uint8_t *codes = static_cast<uint8_t *>(q.codes), *scales = static_cast<uint8_t *>(q.scales);
   const long long pitch = fp4_pitch(q.cols), chunks = fp4_chunks(q.cols, q.format);
   const float inv = 1.0f / q.scale;
@@ -170,11 +178,11 @@ int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda
 #define FX_Q2(DT)                                  \
   do {                                             \
     if (q.format == 16) {                          \
-      if (vec) FX_Q(DT, 16, 16);                   \
-      else FX_Q(DT, 16, 0);                        \
+      if (vec) FX_Q(DT, 16, true);                 \
+      else FX_Q(DT, 16, false);                    \
     } else {                                       \
-      if (vec) FX_Q(DT, 32, 16);                   \
-      else FX_Q(DT, 32, 0);                        \
+      if (vec) FX_Q(DT, 32, true);                 \
+      else FX_Q(DT, 32, false);                    \
     }                                              \
   } while (0)
   if (dtype == FLUX_CUDA_F32) FX_Q2(FLUX_CUDA_F32);
@@ -189,69 +197,85 @@ int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda
 // The values a 4-bit matrix stands for: the product with the matrix's own scale is rounded to f32 and then to the output
 // type, everything else is exact. Same tiling as above; bound by writing the values.
 // ------------------------------------------------------------------------------------------------
-template <int DT, int BLOCK, int ALIGN>
+// Eight codes as f32 values times two factors, one after the other.
+__device__ __forceinline__ void dq_values(uint32_t c, float first, float second, float *v) {
+  uint32_t h[4];
+  fp4_unpack8(c, h);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+    v[2 * j] = f.x * first * second;
+    v[2 * j + 1] = f.y * first * second;
+  }
+}
+
+// VEC: out and its row pitch are multiples of 32 bytes: 16 columns per thread in stores of 32 bytes. Otherwise the lanes of
+// a half-warp take neighbouring columns, so that the stores of an odd pitch still fill whole sectors.
+template <int DT, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t *__restrict__ codes, long long pitch,
                                                                    const uint8_t *__restrict__ scales, long long chunks,
                                                                    int rows, int cols, float scale, void *__restrict__ out,
                                                                    long long ld, int col_tiles, int *sat) {
-  constexpr int CH = Q_COLS / (4 * BLOCK);
-  __shared__ __align__(16) uint8_t fac[CH * 512];
   pdl_launch_dependents();
-  const long long rt = blockIdx.x / col_tiles;
-  const int ct = blockIdx.x % col_tiles;
-  const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
-  const int here = static_cast<int>(rows - rt * Q_ROWS < Q_ROWS ? rows - rt * Q_ROWS : Q_ROWS);
-  const long long c0 = static_cast<long long>(ct) * Q_COLS + cx * 16;
-  const long long chunk = static_cast<long long>(ct) * CH + (threadIdx.x >> 5);
-  if (threadIdx.x < CH * 32)
-    reinterpret_cast<uint4 *>(fac)[threadIdx.x] =
-        chunk < chunks ? __ldg(reinterpret_cast<const uint4 *>(scales + (rt * chunks + chunk) * 512) + (threadIdx.x & 31))
-                       : make_uint4(0, 0, 0, 0);
-  __syncthreads();
+  const int ct = blockIdx.x % col_tiles, rg = blockIdx.x / col_tiles % 4;
+  const long long rt = blockIdx.x / col_tiles / 4;
+  const int cx = threadIdx.x & 15, r32 = rg * 8 + (threadIdx.x >> 4);
+  const long long c0 = static_cast<long long>(ct) * Q_COLS + cx * 16, r0 = rt * 128 + r32;
+  uint2 cd[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    cd[q] = c0 / 2 + 8 <= pitch && r0 + 32 * q < rows
+                ? __ldg(reinterpret_cast<const uint2 *>(codes + (r0 + 32 * q) * pitch + c0 / 2))
+                : make_uint2(0, 0);
+  const long long chunk = c0 / (4 * BLOCK);
+  uint4 f4 = make_uint4(0, 0, 0, 0);
+  if (chunk < chunks && r0 < rows) f4 = __ldg(reinterpret_cast<const uint4 *>(scales + (rt * chunks + chunk) * 512 + r32 * 16));
+  const int sh = (cx * 16 / BLOCK & 3) * 8;
+  const uint32_t fw[4] = {f4.x >> sh, f4.y >> sh, f4.z >> sh, f4.w >> sh};
   float mx = 0.f;
-  if (c0 < cols) {
-#pragma unroll 4
-    for (int it = 0; it < Q_ROWS / 16; ++it) {
-      const int rl = it * 16 + ry;
-      if (rl >= here) break;
-      const long long r = rt * Q_ROWS + rl;
-      const uint2 cd = __ldg(reinterpret_cast<const uint2 *>(codes + r * pitch + c0 / 2));
-      const int b = cx * 16 / BLOCK;
-      const float s = fp4_factor<BLOCK>(fac[(b >> 2) * 512 + (rl & 31) * 16 + (rl >> 5) * 4 + (b & 3)]);
-      // code * e4m3 is exact. A power of two may take a code out of the f32 range that a small scale brings back: then
-      // the scale comes first.
-      const bool scale_first = BLOCK == 32 && fabsf(scale) < 1.0f;
-      const float first = scale_first ? scale : s, second = scale_first ? s : scale;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const long long r = r0 + 32 * q;
+    // code * e4m3 is exact. A power of two may take a code out of the f32 range that a small scale brings back: then the
+    // scale comes first.
+    const float s = fp4_factor<BLOCK>(fw[q] & 0xFFu);
+    const bool scale_first = BLOCK == 32 && fabsf(scale) < 1.0f;
+    const float first = scale_first ? scale : s, second = scale_first ? s : scale;
+    if (VEC && c0 + 16 <= cols) {
+      if (r >= rows) continue;
       float v[16];
+      dq_values(cd[q].x, first, second, v);
+      dq_values(cd[q].y, first, second, v + 8);
+      char *p = reinterpret_cast<char *>(out) + (r * ld + c0) * FP4_SIZE<DT>;
+      uint32_t w[Raw16<DT>::N];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t h[4];
-        fp4_unpack8(k ? cd.y : cd.x, h);
+      for (int k = 0; k < Raw16<DT>::N; ++k)
+        w[k] = DT == FLUX_CUDA_F32 ? __float_as_uint(v[k]) : pack_16x2_t(v[2 * k & 15], v[2 * k + 1 & 15], DT == FLUX_CUDA_F16, mx);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
-          v[8 * k + 2 * j] = f.x * first * second;
-          v[8 * k + 2 * j + 1] = f.y * first * second;
-        }
-      }
-      const long long at = r * ld + c0;
-      if (ALIGN && c0 + 16 <= cols) {
-        if (DT == FLUX_CUDA_F32) {
-          float4 *p = reinterpret_cast<float4 *>(reinterpret_cast<float *>(out) + at);
+      for (int k = 0; k < Raw16<DT>::N; k += 8)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + k * 4), "r"(w[k]), "r"(w[k + 1]),
+                     "r"(w[k + 2]), "r"(w[k + 3]), "r"(w[k + 4]), "r"(w[k + 5]), "r"(w[k + 6]), "r"(w[k + 7])
+                     : "memory");
+    } else if (VEC) {
+      if (r >= rows || c0 >= cols) continue;
+      float v[16];
+      dq_values(cd[q].x, first, second, v);
+      dq_values(cd[q].y, first, second, v + 8);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-        } else {
-          uint4 *p = reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out) + at);
-          uint32_t w[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = pack_16x2_t(v[2 * k], v[2 * k + 1], DT == FLUX_CUDA_F16, mx);
-          p[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          p[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (c0 + k < cols) fp4_store<DT>(out, at + k, v[k], mx);
+      for (int k = 0; k < 16; ++k)
+        if (c0 + k < cols) fp4_store<DT>(out, r * ld + c0 + k, v[k], mx);
+    } else {
+      // lane l of the half-warp takes column l of each of the sixteen lanes' columns in turn
+      const uint32_t mine = threadIdx.x & 16;
+#pragma unroll 4
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t lo = __shfl_sync(0xffffffffu, cd[q].x, mine + k), hi = __shfl_sync(0xffffffffu, cd[q].y, mine + k);
+        const float a = __shfl_sync(0xffffffffu, first, mine + k), b = __shfl_sync(0xffffffffu, second, mine + k);
+        const uint32_t code = ((cx & 8 ? hi : lo) >> (4 * (cx & 7))) & 15;
+        float v[8];
+        dq_values(code, a, b, v);
+        const long long c = static_cast<long long>(ct) * Q_COLS + k * 16 + cx;
+        if (r < rows && c < cols) fp4_store<DT>(out, r * ld + c, v[0], mx);
       }
     }
   }
@@ -260,9 +284,9 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t
 
 int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long long ld, int *sat, cudaStream_t st) {
   const int col_tiles = (q.cols + Q_COLS - 1) / Q_COLS;
-  const long long blocks = fp4_row_tiles(q.rows) * col_tiles;
+  const long long blocks = fp4_row_tiles(q.rows) * 4 * col_tiles;
   const int size = dtype == FLUX_CUDA_F32 ? 4 : 2;
-  const bool vec = !(reinterpret_cast<uintptr_t>(out) & 15) && !((ld * size) & 15);
+  const bool vec = !(reinterpret_cast<uintptr_t>(out) & 31) && !((ld * size) & 31);
   const uint8_t *codes = static_cast<const uint8_t *>(q.codes), *scales = static_cast<const uint8_t *>(q.scales);
   const long long pitch = fp4_pitch(q.cols), chunks = fp4_chunks(q.cols, q.format);
 #define FX_D(DT, BL, AL)                                                                                                   \
@@ -271,11 +295,11 @@ int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long lon
 #define FX_D2(DT)                                  \
   do {                                             \
     if (q.format == 16) {                          \
-      if (vec) FX_D(DT, 16, 16);                   \
-      else FX_D(DT, 16, 0);                        \
+      if (vec) FX_D(DT, 16, true);                 \
+      else FX_D(DT, 16, false);                    \
     } else {                                       \
-      if (vec) FX_D(DT, 32, 16);                   \
-      else FX_D(DT, 32, 0);                        \
+      if (vec) FX_D(DT, 32, true);                 \
+      else FX_D(DT, 32, false);                    \
     }                                              \
   } while (0)
   if (dtype == FLUX_CUDA_F32) FX_D2(FLUX_CUDA_F32);
