@@ -39,21 +39,41 @@ __device__ __forceinline__ void q_expand(uint32_t w, float &lo, float &hi) {
   }
 }
 
-// 16 consecutive elements as 32-bit words, from a 32-byte aligned address.
+// 16 consecutive elements as 32-bit words. From a 32-byte aligned address in loads of 32 bytes; from any other one in the
+// aligned 16-byte pieces that hold them, shifted into place.
 template <int DT>
 struct Raw16 {
   static constexpr int N = DT == FLUX_CUDA_F32 ? 16 : 8;
   uint32_t w[N];
 };
 template <int DT>
-__device__ __forceinline__ void q_load_raw(const void *x, long long i, Raw16<DT> &raw) {
-  const char *p = reinterpret_cast<const char *>(x) + i * FP4_SIZE<DT>;
+__device__ __forceinline__ void q_load_aligned(const char *p, Raw16<DT> &raw) {
 #pragma unroll
   for (int k = 0; k < Raw16<DT>::N; k += 8)
     asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(raw.w[k]), "=r"(raw.w[k + 1]), "=r"(raw.w[k + 2]), "=r"(raw.w[k + 3]), "=r"(raw.w[k + 4]),
                    "=r"(raw.w[k + 5]), "=r"(raw.w[k + 6]), "=r"(raw.w[k + 7])
                  : "l"(p + k * 4));
+}
+// The pieces around [p, p + 16 elements): N / 4 + 1 of them, the last one only if p is not 16-byte aligned.
+template <int DT>
+__device__ __forceinline__ void q_load_shifted(const char *p, Raw16<DT> &raw) {
+  constexpr int N = Raw16<DT>::N;
+  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15;
+  const uint4 *g = reinterpret_cast<const uint4 *>(p - off);
+  uint32_t t[N + 4];
+#pragma unroll
+  for (int k = 0; k <= N / 4; ++k) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (k < N / 4 || off) u = __ldg(g + k);
+    t[4 * k] = u.x, t[4 * k + 1] = u.y, t[4 * k + 2] = u.z, t[4 * k + 3] = u.w;
+  }
+#pragma unroll
+  for (int k = 0; k < N + 2; ++k) t[k] = off & 8 ? t[k + 2] : t[k];
+#pragma unroll
+  for (int k = 0; k < N + 1; ++k) t[k] = off & 4 ? t[k + 1] : t[k];
+#pragma unroll
+  for (int k = 0; k < N; ++k) raw.w[k] = DT == FLUX_CUDA_F32 ? t[k] : __funnelshift_r(t[k], t[k + 1], (off & 2) * 8);
 }
 template <int DT>
 __device__ __forceinline__ void q_expand16(const Raw16<DT> &raw, float (&v)[16]) {
@@ -63,48 +83,90 @@ __device__ __forceinline__ void q_expand16(const Raw16<DT> &raw, float (&v)[16])
     else if (!(k & 1)) q_expand<DT>(raw.w[k / 2], v[k], v[k + 1]);
 }
 
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// The largest of three magnitudes, NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+
 // Codes of 16 columns and the factor byte of their block. For blocks of 32 the two threads of a block exchange their
 // maxima, so the whole warp must call this.
 template <int BLOCK>
 __device__ __forceinline__ uint32_t q_encode(float (&v)[16], float inv_scale, uint2 &codes) {
-  uint32_t top = 0;
+  if (inv_scale != 1.0f) {
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    v[k] *= inv_scale;
-    top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);  // NaN compares above infinity
+    for (int k = 0; k < 16; ++k) v[k] *= inv_scale;
   }
+  float a = fabsf(v[0]);
+#pragma unroll
+  for (int k = 1; k < 15; k += 2) a = max3_abs(a, v[k], v[k + 1]);
+  uint32_t top = __float_as_uint(max3_abs(a, a, v[15])) & 0x7FFFFFFFu;  // NaN compares above infinity
   if (BLOCK == 32) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   const bool bad = top >= 0x7F800000u;
+  if (bad) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = 0.f;
+  }
   uint32_t byte;
+  float q[16];
   if (BLOCK == 32) {
     const int e = static_cast<int>(top >> 23) - 2;
     byte = bad ? 255u : static_cast<uint32_t>(e > 0 ? e : 0);
     const float r = bad ? 0.f : __uint_as_float((254u - byte) << 23);  // 2^-(byte - 127): the quotient is exact
+    const uint64_t r2 = f2_pack(r, r);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = bad ? 0.f : v[k] * r;
+    for (int k = 0; k < 16; k += 2) f2_unpack(f2_mul(f2_pack(v[k], v[k + 1]), r2), q[k], q[k + 1]);
   } else {
-    // a / 6 rounded to odd: truncated, with the lowest bit set where something was cut off; rounding that to e4m3 is
+    // a / 6 rounded to odd (truncated, with the lowest bit set where something was cut off): rounding that to e4m3 is
     // rounding the exact quotient
-    const float a = __uint_as_float(top);
-    float q = __fdiv_rz(a, 6.0f);
-    if (__fmaf_rn(-q, 6.0f, a) != 0.f) q = __uint_as_float(__float_as_uint(q) | 1u);
+    a = __uint_as_float(bad ? 0u : top);
+    float t = a * (1.0f / 6.0f);  // within one unit of a / 6; the residual's sign tells on which side
+    const float rest = __fmaf_rn(-t, 6.0f, a);
+    uint32_t bits = __float_as_uint(t);
+    if (rest < 0.f) bits -= 1;
+    if (rest != 0.f) bits |= 1;
+    t = __uint_as_float(bits);
     uint16_t e;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(e) : "f"(0.f), "f"(q));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(e) : "f"(0.f), "f"(t));
     byte = bad ? 0x7Fu : (e & 0xFFu);
-    const float s = bad ? 0.f : fp4_factor<16>(byte);
-    const float r = s > 0.f ? __frcp_rn(s) : 0.f;
+    const float s = fp4_factor<16>(e & 0xFFu);
+    float r = 0.f;
+    if (s > 0.f) {  // one Newton step: the correctly rounded reciprocal for every one of the 126 factors
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+      r = __fmaf_rn(__fmaf_rn(-s, r, 1.0f), r, r);
+    }
     // Markstein's correction: with r the correctly rounded reciprocal, fma(fma(-q, s, x), r, q) is the correctly
     // rounded quotient
+    const uint64_t r2 = f2_pack(r, r), s2 = f2_pack(-s, -s);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float x = bad ? 0.f : v[k];
-      const float q0 = x * r;
-      v[k] = __fmaf_rn(__fmaf_rn(-q0, s, x), r, q0);
+    for (int k = 0; k < 16; k += 2) {
+      const uint64_t x2 = f2_pack(v[k], v[k + 1]), q2 = f2_mul(x2, r2);
+      f2_unpack(f2_fma(f2_fma(q2, s2, x2), r2, q2), q[k], q[k + 1]);
     }
   }
   float lo[8], hi[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) lo[k] = v[k], hi[k] = v[8 + k];
+  for (int k = 0; k < 8; ++k) lo[k] = q[k], hi[k] = q[8 + k];
   codes = make_uint2(fp4_pack8(lo), fp4_pack8(hi));
   return byte;
 }
@@ -120,12 +182,22 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_quantize_kernel(const void *__r
   const long long rt = blockIdx.x / col_tiles / 4;
   const int cx = threadIdx.x & 15, r32 = rg * 8 + (threadIdx.x >> 4);
   const long long c0 = static_cast<long long>(ct) * Q_COLS + cx * 16, r0 = rt * 128 + r32;
-  const bool whole = VEC && c0 + 16 <= cols;
+  const char *base = static_cast<const char *>(x), *end = base + ((rows - 1) * ldx + cols) * FP4_SIZE<DT>;
   Raw16<DT> raw[4];
-  if (whole) {
+  bool whole[4];  // all 16 elements are in `raw`
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (r0 + 32 * q < rows) q_load_raw<DT>(x, (r0 + 32 * q) * ldx + c0, raw[q]);
+  for (int q = 0; q < 4; ++q) {
+    const char *p = base + ((r0 + 32 * q) * ldx + c0) * FP4_SIZE<DT>;
+    whole[q] = r0 + 32 * q < rows && c0 + 16 <= cols;
+    if (VEC) {
+      if (whole[q]) q_load_aligned<DT>(p, raw[q]);
+    } else {
+      // the 16-byte pieces around the elements must lie inside the matrix themselves
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15);
+      whole[q] = whole[q] && lo >= reinterpret_cast<uintptr_t>(base) &&
+                 ((reinterpret_cast<uintptr_t>(p) + 16 * FP4_SIZE<DT> + 15) & ~uintptr_t(15)) <= reinterpret_cast<uintptr_t>(end);
+      if (whole[q]) q_load_shifted<DT>(p, raw[q]);
+    }
   }
   uint32_t word[4];  // the factors of this lane's chunk of four blocks
 #pragma unroll
@@ -137,7 +209,7 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_quantize_kernel(const void *__r
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k] = 0.f;
     if (live) {
-      if (whole) {
+      if (whole[q]) {
         q_expand16<DT>(raw[q], v);
       } else {
         const long long at = (r0 + 32 * q) * ldx + c0;
@@ -209,8 +281,17 @@ __device__ __forceinline__ void dq_values(uint32_t c, float first, float second,
   }
 }
 
+template <int DT>
+struct OutElement {
+  using T = uint16_t;
+};
+template <>
+struct OutElement<FLUX_CUDA_F32> {
+  using T = uint32_t;
+};
+
 // VEC: out and its row pitch are multiples of 32 bytes: 16 columns per thread in stores of 32 bytes. Otherwise the lanes of
-// a half-warp take neighbouring columns, so that the stores of an odd pitch still fill whole sectors.
+// a warp store neighbouring columns, so that the stores of an odd pitch still fill whole sectors.
 template <int DT, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t *__restrict__ codes, long long pitch,
                                                                    const uint8_t *__restrict__ scales, long long chunks,
@@ -241,6 +322,7 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t
     const float s = fp4_factor<BLOCK>(fw[q] & 0xFFu);
     const bool scale_first = BLOCK == 32 && fabsf(scale) < 1.0f;
     const float first = scale_first ? scale : s, second = scale_first ? s : scale;
+    float top = 0.f;
     if (VEC && c0 + 16 <= cols) {
       if (r >= rows) continue;
       float v[16];
@@ -265,18 +347,31 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t
       for (int k = 0; k < 16; ++k)
         if (c0 + k < cols) fp4_store<DT>(out, r * ld + c0 + k, v[k], mx);
     } else {
-      // lane l of the half-warp takes column l of each of the sixteen lanes' columns in turn
-      const uint32_t mine = threadIdx.x & 16;
-#pragma unroll 4
-      for (int k = 0; k < 16; ++k) {
-        const uint32_t lo = __shfl_sync(0xffffffffu, cd[q].x, mine + k), hi = __shfl_sync(0xffffffffu, cd[q].y, mine + k);
-        const float a = __shfl_sync(0xffffffffu, first, mine + k), b = __shfl_sync(0xffffffffu, second, mine + k);
-        const uint32_t code = ((cx & 8 ? hi : lo) >> (4 * (cx & 7))) & 15;
-        float v[8];
-        dq_values(code, a, b, v);
-        const long long c = static_cast<long long>(ct) * Q_COLS + k * 16 + cx;
-        if (r < rows && c < cols) fp4_store<DT>(out, r * ld + c, v[0], mx);
+      // through shared memory, so that the lanes of a warp store neighbouring elements of a row
+      using E = typename OutElement<DT>::T;
+      __shared__ __align__(16) E stage[Q_THREADS / 32][2][Q_COLS];
+      float v[16];
+      dq_values(cd[q].x, first, second, v);
+      dq_values(cd[q].y, first, second, v + 8);
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+      uint4 *mine = reinterpret_cast<uint4 *>(&stage[warp][lane >> 4][cx * 16]);
+      uint32_t w[Raw16<DT>::N];
+#pragma unroll
+      for (int k = 0; k < Raw16<DT>::N; ++k)
+        w[k] = DT == FLUX_CUDA_F32 ? __float_as_uint(v[k]) : pack_16x2_t(v[2 * k & 15], v[2 * k + 1 & 15], DT == FLUX_CUDA_F16, top);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < Raw16<DT>::N / 4; ++k) mine[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long row = r - (threadIdx.x >> 4 & 1) + h, c = static_cast<long long>(ct) * Q_COLS + lane;
+        E *p = reinterpret_cast<E *>(out) + row * ld + c;
+#pragma unroll
+        for (int k = 0; k < Q_COLS / 32; ++k)
+          if (row < rows && c + 32 * k < cols) p[32 * k] = stage[warp][h][32 * k + lane];
       }
+      if (r < rows && c0 < cols) mx = fmaxf(mx, top);
     }
   }
   sat_report(sat, DT == FLUX_CUDA_F16, mx);
