@@ -37,10 +37,11 @@ int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda
 int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long long ld, int *sat, cudaStream_t st);
 int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st);
 int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const flux_cuda_fp4 &w, void *out, int dtype,
-                    long long ld_out, int num_sms, int *sat, cudaStream_t st);
+                    long long ld_out, int device, int *sat, cudaStream_t st);
 int fp4_gemm_init();  // opts the product kernels into large shared memory
+int fp4_gemv_init(int device);  // counts the clusters that the current device holds
 
-static constexpr int FP4_GEMV_MAX_ROWS = 16;
+static constexpr int FP4_GEMV_MAX_ROWS = 16, FP4_GEMV_MAX_COLS = 65536;  // what eight SMs' shared memory holds of x
 
 template <int DT>
 constexpr int FP4_SIZE = DT == FLUX_CUDA_F32 ? 4 : 2;
@@ -97,6 +98,32 @@ __device__ __forceinline__ float fp4_factor(uint32_t byte) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(byte)));
   return __half2float(__ushort_as_half(static_cast<uint16_t>(h & 0xFFFFu)));
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// A word of another CTA's shared memory (an address from map_to_cta).
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 }  // namespace fx

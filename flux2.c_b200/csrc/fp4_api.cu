@@ -125,13 +125,14 @@ int flux_cuda_gemv_fp4(flux_cuda_ctx *ctx, const void *x, int x_dtype, long long
   int rc = check_matrix(op, "w", w);
   if (rc) return rc;
   if (rows < 0 || rows > FP4_GEMV_MAX_ROWS) return refuse(op, "takes 0 to 16 rows");
+  if (w->cols > FP4_GEMV_MAX_COLS) return refuse(op, "takes up to 65536 columns");
   if ((rc = check_plain(op, "x", x, x_dtype, ldx, rows, w->cols)) ||
       (rc = check_plain(op, "out", out, dtype, ld_out, rows, w->rows)))
     return rc;
   if (!ctx) return refuse(op, "null context");
   if (rows == 0 || w->rows == 0) return FLUX_CUDA_OK;
   OnDevice on(ctx->device);
-  return finish(op, launch_gemv_fp4(x, x_dtype, ldx, rows, *w, out, dtype, ld_out, ctx->num_sms, ctx->err_dev + 1,
+  return finish(op, launch_gemv_fp4(x, x_dtype, ldx, rows, *w, out, dtype, ld_out, ctx->device, ctx->err_dev + 1,
                                     ctx->stream));
 }
 

@@ -1,171 +1,457 @@
 // A few rows of f32 / f16 / bf16 times a 4-bit matrix: out[m, n] = w.scale * sum_k x[m, k] w[n, k], the activations not
-// quantised. The form for single tokens and for the modulation vectors of a schedule; bound by reading the packed
-// weights once (0.56 bytes per weight).
+// quantised. The form for single tokens and for the modulation vectors of a schedule. Bound by reading the packed weights
+// once (0.56 bytes per weight) and by decoding them.
 //
-// One warp takes the four weight rows r, r + 32, r + 64, r + 96 of a 128-row tile, because one 16-byte piece of a factor
-// tile holds the factors of exactly these rows for four blocks; a lane takes 32 consecutive codes (16 bytes) of each per
-// step, so a step of the warp covers 1024 codes of four rows. x is laid out once per block in shared memory as f32, in
-// the order in which the lanes read it ([piece of 4][lane]: no bank conflicts), for up to four rows of x at a time; more
-// rows are further blocks, whose weights then come from L2. Sums are f32: per lane over its codes, then over the warp.
+// Decoding: a code and its factor are an exact bf16 value (at most six significant bits). The three magnitude bits of a
+// code, put at the border of a bf16's exponent and mantissa, are the code's value times 2^-126 (the code for 0.5 becomes a
+// subnormal), so a mask, an integer multiplication, a mask and one packed multiplication by factor * 2^110 (blocks of 32:
+// 2^(e + 126)) make two weights. Multiplying in f32 instead takes two conversions and one multiply-add per weight and row of x: measured 17 us
+// for one row and 36 for four (19456 x 2560), bound by instructions.
+//
+// Products: mma.sync m16n8k16 on bf16, 16 weight rows by up to 8 rows of x, f32 sums; x is split exactly into bf16 parts
+// (bf16 1, f16 2, f32 3), so every product is exact and up to 8 rows of x share one decoding. (tcgen05 wants its operands in
+// shared memory; decoded weights go from registers to the multiplication here.)
+//
+// A warp takes 32 weight rows at a time (a "unit": rows r + 32 q, r = 8 neighbours, q = 0..3, because one 16-byte piece of
+// a factor tile holds the factors of exactly the rows r + 32 q for four blocks) in steps of 256 columns, a 128-byte line of
+// each row: a lane loads twice 32 consecutive codes of its four rows, and because sums do not care for order, those are its
+// columns in the multiplication too. The loads go to a ring in shared memory, asynchronously and each lane to places of its
+// own, so that a step is on its way while one is computed without costing registers or barriers; 64 bytes of a row at a
+// time into registers came to 2.1 TB/s. x lies in shared memory in the order of the multiplication's registers. K is split among the CTAs of a cluster, so that
+// x fits and the units of a cluster are many enough to be shared out evenly; the warps of a CTA take equal stretches
+// of its (unit, step) pairs, wherever these begin and end. Partial sums are added in a fixed order through (distributed)
+// shared memory: no workspace, no atomics, the same bits every time.
 #include "fp4.cuh"
+#include "launch.cuh"
 
 namespace fx {
 
-static constexpr int V_THREADS = 512;
-static constexpr int V_SMEM_MAX = 200 * 1024;
+static constexpr int V_WARPS = 16, V_THREADS = 32 * V_WARPS;  // one block per SM
+static constexpr int V_STEP_BYTES = 2 * 5 * 512;               // a warp's codes and factors of a step
+static constexpr int V_RING = 2 * V_WARPS * V_STEP_BYTES;      // two steps per warp
+static constexpr int V_SMEM_MAX = 227 * 1024 - V_RING;         // what is left for x and the sums
 
-__device__ __forceinline__ float v_load(const void *x, int dt, long long i) {
-  if (dt == FLUX_CUDA_F32) return reinterpret_cast<const float *>(x)[i];
-  const uint16_t h = reinterpret_cast<const uint16_t *>(x)[i];
-  return dt == FLUX_CUDA_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+struct GemvFp4Params {
+  const void *x;
+  int x_vec;  // x and its row pitch are multiples of 16 bytes
+  long long ldx;
+  int rows, group;  // rows of x; rows of x per block
+  const uint8_t *codes, *scales;
+  long long pitch, chunks;
+  float scale;
+  int N, K, steps;  // steps of 256 columns
+  int kparts;       // K is split among this many CTAs of a cluster
+  int part_steps;   // most steps of a CTA
+  int clusters;
+  long long units;
+  void *out;
+  int dt;
+  long long ld;
+  int *sat;
+  uint2 by;  // 2^12 + 2^6 and 2^8 + 2^2 (v_place); not constants, which the compiler would take apart into shifts
+};
+
+// Where a lane's pieces of the next step lie. Rows past the last one read it instead (their sums are dropped).
+struct VRows {
+  const uint8_t *codes[4], *factors;
+};
+template <int BLOCK>
+__device__ __forceinline__ VRows v_rows(const GemvFp4Params &P, long long unit, int step, int lane) {
+  const int g = lane >> 2, t = lane & 3, r32 = static_cast<int>(unit & 3) * 8 + g;
+  const long long n0 = (unit >> 2) * 128 + r32;
+  VRows r;
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    r.codes[q] = P.codes + (n0 + 32 * q < P.N ? n0 + 32 * q : P.N - 1) * P.pitch + step * 128 + t * 16;
+  r.factors = P.scales + ((unit >> 2) * P.chunks + step * (64 / BLOCK) + t * 8 / BLOCK) * 512 + r32 * 16;
+  return r;
+}
+// 16 bytes from global to shared memory, asynchronously; zeros where there is nothing to read.
+__device__ __forceinline__ void v_copy16(uint32_t dst, const uint8_t *src, bool in) {
+  if (in) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+}
+// A step of a unit into this lane's places, [half of the step][4 rows of codes, factors][lane], and on to the next step.
+// left: bytes of codes and chunks of factors from the step's first column to the end of the row.
+template <int BLOCK>
+__device__ __forceinline__ void v_fetch(uint32_t dst, VRows &r, int step, int t, int code_end, int factor_end) {
+  const int left = code_end - step * 128 - t * 16, chunks = factor_end - step * (64 / BLOCK) - t * 8 / BLOCK;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // half a step is 32 / BLOCK chunks: two of 64 columns, or one of 128
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v_copy16(dst + (h * 5 + q) * 512, r.codes[q] + h * 64, left > h * 64);
+    v_copy16(dst + (h * 5 + 4) * 512, r.factors + h * (32 / BLOCK) * 512, chunks > h * (32 / BLOCK));
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) r.codes[q] += 128;
+  r.factors += (64 / BLOCK) * 512;
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ uint4 v_ring(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 
-// S rows of x per block (blockIdx.y * S ...). STAGED: x lies in shared memory; otherwise (K too long) it is read from
-// global memory.
-template <int S, int BLOCK, bool STAGED>
-__global__ void __launch_bounds__(V_THREADS) gemv_fp4_kernel(const void *__restrict__ x, int x_dt, long long ldx, int rows,
-                                                             const uint8_t *__restrict__ codes, long long pitch,
-                                                             const uint8_t *__restrict__ scales, long long chunks,
-                                                             float scale, int N, int K, void *__restrict__ out, int dt,
-                                                             long long ld, int *sat) {
-  extern __shared__ float4 xs[];  // [S][steps][8][32]
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int steps = (K + 1023) / 1024;
-  const int m0 = blockIdx.y * S;
-  if (STAGED) {
-    float *f = reinterpret_cast<float *>(xs);
-    for (int i = threadIdx.x; i < S * steps * 1024; i += V_THREADS) {
-      // destination order: [row][step][piece j][lane][4]
-      const int e = i & 3, l = (i >> 2) & 31, j = (i >> 7) & 7, st = (i >> 10) % steps, s = (i >> 10) / steps;
-      const long long k = static_cast<long long>(st) * 1024 + l * 32 + j * 4 + e;
-      f[i] = (m0 + s < rows && k < K) ? v_load(x, x_dt, (m0 + s) * ldx + k) : 0.f;
-    }
-    __syncthreads();
+__device__ __forceinline__ uint32_t v_mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Eight codes to four bf16 pairs (codes i and i + 4) times m (a pair of equal factors). One multiplication by 2^a + 2^b puts
+// a masked code's sign and its magnitude where they belong at once; the copies that land elsewhere are masked off. (With a
+// shift and a mask for each the decoding was bound by the integer pipe: 275 of its instructions per 128 codes and lane.)
+__device__ __forceinline__ uint32_t v_place(uint32_t code, uint32_t by) { return (code * by) & 0x81C081C0u; }
+__device__ __forceinline__ void v_decode(uint32_t w, uint32_t m, uint2 by, uint32_t (&p)[4]) {
+  const uint32_t v = w >> 8;
+  p[0] = v_mul2(v_place(w & 0x000F000Fu, by.x), m);
+  p[1] = v_mul2(v_place(w & 0x00F000F0u, by.y), m);
+  p[2] = v_mul2(v_place(v & 0x000F000Fu, by.x), m);
+  p[3] = v_mul2(v_place(v & 0x00F000F0u, by.y), m);
+}
+__device__ __forceinline__ void v_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same onto zeros: the start of a chain.
+__device__ __forceinline__ void v_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// The exact bf16 parts of a value, the largest first (8 bits of the magnitude each).
+template <int PARTS>
+__device__ __forceinline__ void v_split(float x, uint32_t (&p)[PARTS]) {
+  const bool finite = (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
+  if (!finite && x != x) x = __uint_as_float(0x7FC00000u);
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const uint32_t top = __float_as_uint(x) & 0xFFFF0000u;
+    p[i] = top >> 16;
+    x = finite ? x - __uint_as_float(top) : 0.f;
   }
-  const long long quads = (static_cast<long long>(N) + 127) / 128 * 32;
-  float mx = 0.f;
-  for (long long t = blockIdx.x * static_cast<long long>(V_THREADS / 32) + (threadIdx.x >> 5); t < quads;
-       t += static_cast<long long>(gridDim.x) * (V_THREADS / 32)) {
-    const long long n0 = t / 32 * 128 + t % 32;  // rows n0 + 32 q
-    if (n0 >= N) continue;
-    float acc[4][S];
+}
+
+// Elements of x, whose type has PARTS parts; eight of them from a 16-byte aligned address.
+template <int PARTS>
+__device__ __forceinline__ float v_load(const void *x, long long i) {
+  if (PARTS == 3) return __ldg(reinterpret_cast<const float *>(x) + i);
+  const uint16_t h = __ldg(reinterpret_cast<const uint16_t *>(x) + i);
+  return PARTS == 2 ? __half2float(__ushort_as_half(h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+}
+template <int PARTS>
+__device__ __forceinline__ void v_load8(const void *x, long long i, float (&v)[8]) {
+  if (PARTS == 3) {
+    const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(x) + i);
+    const float4 a = __ldg(p), b = __ldg(p + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(x) + i));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int j = 0; j < 4; ++j) {
+      if (PARTS == 2) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+        v[2 * j] = f.x, v[2 * j + 1] = f.y;
+      } else {
+        v[2 * j] = bf16_lo(w[j]), v[2 * j + 1] = bf16_hi(w[j]);
+      }
+    }
+  }
+}
+
+// NH: 8 NH rows of x per block at most (group of them); PARTS: bf16 parts of x.
+template <int NH, int PARTS, int BLOCK>
+__global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_constant__ GemvFp4Params P) {
+  // the ring, then x [2 part_steps][PARTS][4][group][4], then sums [units + 2 V_WARPS][group][32]
+  extern __shared__ uint4 shared[];
+  uint4 *xs = shared + V_RING / 16;
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int part = blockIdx.x % P.kparts, cluster = blockIdx.x / P.kparts;
+  const int G = P.group, m0 = blockIdx.y * G;
+  const int s0 = static_cast<int>(static_cast<long long>(P.steps) * part / P.kparts),
+            s1 = static_cast<int>(static_cast<long long>(P.steps) * (part + 1) / P.kparts), L = s1 - s0;
+  const long long u0 = P.units * cluster / P.clusters;
+  const int nu = static_cast<int>(P.units * (cluster + 1) / P.clusters - u0);
+  float *sums = reinterpret_cast<float *>(xs + 2 * P.part_steps * PARTS * 16 * G);
+
+  // this warp's stretch of the nu * L pairs, unit by unit
+  auto begin_of = [&](int w) { return static_cast<int>(static_cast<long long>(nu) * L * w / V_WARPS); };
+  const int first = begin_of(warp), last = begin_of(warp + 1);
+  int u = first / L, st = first - u * L;
+  VRows rows = v_rows<BLOCK>(P, u0 + (u < nu ? u : 0), s0 + st, lane);
+  const int code_end = static_cast<int>(P.pitch), factor_end = static_cast<int>(P.chunks);
+  // lanes beyond the rows of x repeat the last one: the sums they take part in are dropped
+  int x_lane[NH];
 #pragma unroll
-      for (int s = 0; s < S; ++s) acc[q][s] = 0.f;
-    for (int st = 0; st < steps; ++st) {
-      const long long byte = st * 512LL + lane * 16;
-      uint4 w[4];
+  for (int nh = 0; nh < NH; ++nh) x_lane[nh] = (g + 8 * nh < G ? g + 8 * nh : G - 1) * 4 + t;
+  const uint32_t ring = smem_u32(shared) + warp * 2 * V_STEP_BYTES + lane * 16;
+  if (first < last) v_fetch<BLOCK>(ring, rows, s0 + st, t, code_end, factor_end);  // the weights do not wait for x
+  for (int i = threadIdx.x; i < 2 * L * 16 * G; i += V_THREADS) {  // eight consecutive columns of a row
+    const int c8 = i % (2 * L * 16), m = i / (2 * L * 16);
+    const int sx = c8 >> 4, tt = (c8 >> 2) & 3, jj = c8 & 3;
+    const long long k = s0 * 256LL + sx * 128 + tt * 32 + jj * 8, at = (m0 + m) * P.ldx + k;
+    uint32_t p[8][PARTS];
+    float v[8];
+    if (P.x_vec && m0 + m < P.rows && k + 8 <= P.K) {
+      v_load8<PARTS>(P.x, at, v);
+    } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        w[q] = (byte < pitch && n0 + 32 * q < N) ? __ldg(reinterpret_cast<const uint4 *>(codes + (n0 + 32 * q) * pitch + byte))
-                                                 : make_uint4(0, 0, 0, 0);
-      // 32 codes are two blocks of 16 (half of a factor word) or one of 32 (a quarter)
-      const long long blk = (st * 1024LL + lane * 32) / BLOCK;
-      uint4 sf = make_uint4(0, 0, 0, 0);
-      if (blk / 4 < chunks)
-        sf = __ldg(reinterpret_cast<const uint4 *>(scales + ((n0 / 128) * chunks + blk / 4) * 512 + (n0 % 32) * 16));
-      const int sh = static_cast<int>(blk & 3) * 8;
-      const uint32_t fw[4] = {sf.x >> sh, sf.y >> sh, sf.z >> sh, sf.w >> sh};
+      for (int e = 0; e < 8; ++e) v[e] = m0 + m < P.rows && k + e < P.K ? v_load<PARTS>(P.x, at + e) : 0.f;
+    }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {  // 16 codes each
-        float4 xv[S][4];
+    for (int e = 0; e < 8; ++e) v_split<PARTS>(v[e], p[e]);
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+    for (int h = 0; h < PARTS; ++h)  // columns i and i + 4 in a register, as the codes are decoded
+      xs[(((sx * PARTS + h) * 4 + jj) * G + m) * 4 + tt] = make_uint4(p[0][h] | p[4][h] << 16, p[1][h] | p[5][h] << 16,
+                                                                      p[2][h] | p[6][h] << 16, p[3][h] | p[7][h] << 16);
+  }
+  __syncthreads();
+
+  for (int at = first; at < last; ++u) {
+    const bool begins = st == 0;
+    const int stop = st + (last - at) < L ? st + (last - at) : L;
+    float d[2][NH][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (STAGED) {
-              xv[s][j] = xs[((s * steps + st) * 8 + half * 4 + j) * 32 + lane];
-            } else {
-              float e[4];
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const long long k = st * 1024LL + lane * 32 + half * 16 + j * 4 + i;
-                e[i] = (m0 + s < rows && k < K) ? v_load(x, x_dt, (m0 + s) * ldx + k) : 0.f;
-              }
-              xv[s][j] = make_float4(e[0], e[1], e[2], e[3]);
-            }
-          }
+      for (int h = 0; h < NH; ++h) d[a][h][0] = d[a][h][1] = d[a][h][2] = d[a][h][3] = 0.f;
+    // a unit that this warp does not do alone: its sums go to a place of the warp's own, one for the stretch's first unit
+    // and one for its last
+    float *mine = sums + (begins && stop == L ? u : nu + 2 * warp + (at == first ? 0 : 1)) * G * 32;
+    for (; st < stop; ++st, ++at) {
+      if (at + 1 < last) {
+        if (st + 1 == L) rows = v_rows<BLOCK>(P, u0 + u + 1, s0, lane);
+        v_fetch<BLOCK>(ring + ((at + 1 - first) & 1) * V_STEP_BYTES, rows, s0 + (st + 1 == L ? 0 : st + 1), t, code_end, factor_end);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      }
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+      const uint32_t mine_at = ring + ((at - first) & 1) * V_STEP_BYTES + half * 5 * 512;
+      uint4 cur[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) cur[q] = v_ring(mine_at + q * 512);
+      const uint4 f4 = v_ring(mine_at + 4 * 512);
+      // this lane's factors: two blocks of 16 per row (half of a factor word), or one of 32 (a quarter of it)
+      const uint32_t fw[4] = {f4.x, f4.y, f4.z, f4.w};
+      uint32_t m[4][2];
+      uint32_t over[4];
+      bool wide = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (BLOCK == 16) {
+          uint32_t h;
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(fw[q] >> (t & 1) * 16)));
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+          m[q][0] = __byte_perm(__float_as_uint(f.x * 0x1p110f), 0, 0x3232);
+          m[q][1] = __byte_perm(__float_as_uint(f.y * 0x1p110f), 0, 0x3232);
+        } else {
+          const uint32_t b = fw[q] >> t * 8 & 0xFFu;
+          const uint32_t one = b == 255u ? 0x7FC0u : (min(b, 128u) + 126u) << 7;  // 2^(min(e, 1) + 126)
+          m[q][0] = m[q][1] = one * 0x10001u;
+          over[q] = ((b > 128u && b < 255u ? b - 1u : 127u) << 7) * 0x10001u;  // the rest of a factor above 2: 2^(e - 1)
+          wide |= b > 128u;
+        }
+      }
+      if (BLOCK == 32) wide = __any_sync(0xffffffffu, wide);
+      const uint4 *xp = xs + (2 * st + half) * PARTS * 16 * G;
+      // The instruction truncates its sums: chains of more than 128 columns are added with rounding. (One chain over all of
+      // K was 2.8e-6 off, relative, at K = 9216.)
+      float e[2][NH][4];
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+        uint32_t a[4][4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float f = fp4_factor<BLOCK>((BLOCK == 16 ? fw[q] >> (half * 8) : fw[q]) & 0xFFu);
-          float part[S];
+          const uint32_t w = jj == 0 ? cur[q].x : jj == 1 ? cur[q].y : jj == 2 ? cur[q].z : cur[q].w;
+          v_decode(w, m[q][jj >> 1], P.by, a[q]);
+          if (BLOCK == 32 && wide) {
 #pragma unroll
-          for (int s = 0; s < S; ++s) part[s] = 0.f;
+            for (int i = 0; i < 4; ++i) a[q][i] = v_mul2(a[q][i], over[q]);
+          }
+        }
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t word = half == 0 ? (c == 0 ? w[q].x : w[q].y) : (c == 0 ? w[q].z : w[q].w);
-            uint32_t h[4];
-            fp4_unpack8(word, h);
+        for (int h = 0; h < PARTS; ++h)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h[2 * j]));
-              const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h[2 * j + 1]));
+          for (int nh = 0; nh < NH; ++nh) {
+            const uint4 b = xp[(h * 4 + jj) * G * 4 + x_lane[nh]];
 #pragma unroll
-              for (int s = 0; s < S; ++s) {
-                const float4 v = xv[s][2 * c + j];
-                part[s] = fmaf(a.x, v.x, part[s]);
-                part[s] = fmaf(a.y, v.y, part[s]);
-                part[s] = fmaf(b.x, v.z, part[s]);
-                part[s] = fmaf(b.y, v.w, part[s]);
-              }
+            for (int tile = 0; tile < 2; ++tile) {
+              if (jj + h == 0) v_mma0(e[tile][nh], a[2 * tile][0], a[2 * tile + 1][0], a[2 * tile][1], a[2 * tile + 1][1], b.x, b.y);
+              else v_mma(e[tile][nh], a[2 * tile][0], a[2 * tile + 1][0], a[2 * tile][1], a[2 * tile + 1][1], b.x, b.y);
+              v_mma(e[tile][nh], a[2 * tile][2], a[2 * tile + 1][2], a[2 * tile][3], a[2 * tile + 1][3], b.z, b.w);
             }
           }
+      }
 #pragma unroll
-          for (int s = 0; s < S; ++s) acc[q][s] = fmaf(f, part[s], acc[q][s]);
-        }
+      for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[tile][nh][i] += e[tile][nh][i];
       }
     }
+    st = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const float v = warp_sum(acc[q][s]) * scale;
-        const long long n = n0 + 32 * q;
-        if (lane == 0 && n < N && m0 + s < rows) {
-          const long long at = (m0 + s) * ld + n;
-          if (dt == FLUX_CUDA_F32) fp4_store<FLUX_CUDA_F32>(out, at, v, mx);
-          else if (dt == FLUX_CUDA_F16) fp4_store<FLUX_CUDA_F16>(out, at, v, mx);
-          else fp4_store<FLUX_CUDA_BF16>(out, at, v, mx);
+      for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int m = nh * 8 + 2 * t + (i & 1), q = 2 * tile + (i >> 1);
+          if (m < G) mine[m * 32 + q * 8 + g] = d[tile][nh][i];
         }
-      }
   }
-  sat_report(sat, dt == FLUX_CUDA_F16, mx);
+  __syncthreads();
+  // units in pieces: the pieces in the order of the warps (unit i is pairs [i L, i L + L))
+  for (int i = warp; i < nu; i += V_WARPS) {
+    const int lo = i * L, hi = lo + L;
+    int w0 = static_cast<int>(static_cast<long long>(lo) * V_WARPS / (nu * L));
+    while (w0 + 1 < V_WARPS && begin_of(w0 + 1) <= lo) ++w0;
+    if (begin_of(w0) <= lo && begin_of(w0 + 1) >= hi) continue;  // one warp's alone
+    for (int m = 0; m < G; ++m) {
+      float y = 0.f;
+      for (int w = w0; w < V_WARPS && begin_of(w) < hi; ++w)
+        if (begin_of(w) < begin_of(w + 1)) y += sums[((nu + 2 * w + (begin_of(w) >= lo ? 0 : 1)) * G + m) * 32 + lane];
+      sums[(i * G + m) * 32 + lane] = y;
+    }
+  }
+  // and the parts in the order of the cluster's CTAs
+  if (P.kparts > 1) cluster_sync_all();
+  else __syncthreads();
+  float mx = 0.f;
+  const int count = nu * G * 32;
+  for (int i = part * V_THREADS + threadIdx.x; i < count; i += P.kparts * V_THREADS) {
+    const int rl = i & 31, m = (i >> 5) % G, u = (i >> 5) / G;
+    float y = 0.f;
+    if (P.kparts > 1) {
+      const uint32_t at = smem_u32(sums + i);
+      float p[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < P.kparts) p[c] = ld_cluster_f32(map_to_cta(at, c));
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < P.kparts) y += p[c];
+    } else {
+      y = sums[i];
+    }
+    const long long unit_i = u0 + u, n = (unit_i >> 2) * 128 + (unit_i & 3) * 8 + (rl & 7) + 32 * (rl >> 3);
+    if (n < P.N && m0 + m < P.rows) {
+      if (BLOCK == 16) y *= 65536.0f;  // the factors went in as factor * 2^110, against codes * 2^-126
+      y *= P.scale;
+      const long long at = (m0 + m) * P.ld + n;
+      if (P.dt == FLUX_CUDA_F32) fp4_store<FLUX_CUDA_F32>(P.out, at, y, mx);
+      else if (P.dt == FLUX_CUDA_F16) fp4_store<FLUX_CUDA_F16>(P.out, at, y, mx);
+      else fp4_store<FLUX_CUDA_BF16>(P.out, at, y, mx);
+    }
+  }
+  sat_report(P.sat, P.dt == FLUX_CUDA_F16, mx);
+  if (P.kparts > 1) cluster_sync_all();  // nobody leaves while another CTA still reads its sums
 }
 
-template <int S, int BLOCK, bool STAGED>
-static cudaError_t v_launch(dim3 grid, size_t smem, cudaStream_t st, const void *x, int x_dt, long long ldx, int rows,
-                            const flux_cuda_fp4 &w, void *out, int dt, long long ld, int *sat) {
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(gemv_fp4_kernel<S, BLOCK, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         V_SMEM_MAX);
-    if (e != cudaSuccess) return e;
+// Clusters of 1, 2, 4 and 8 blocks that a device holds at once, one block per SM (the GPCs' numbers of SMs are no multiples of
+// eight, so they are fewer than the SMs make).
+static int g_clusters[64][4];
+int fp4_gemv_init(int device) {
+  if (device < 0 || device >= 64) return -1;
+  auto *kernel = gemv_fp4_kernel<1, 1, 16>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, V_RING + V_SMEM_MAX) != cudaSuccess) return -2;
+  for (int i = 0; i < 4; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(148 << i);
+    cfg.gridDim.x = (cfg.gridDim.x >> i) << i;
+    cfg.blockDim = dim3(V_THREADS);
+    cfg.dynamicSmemBytes = V_RING + V_SMEM_MAX;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1 << i;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return -2;
+    g_clusters[device][i] = n;
   }
-  gemv_fp4_kernel<S, BLOCK, STAGED><<<grid, V_THREADS, smem, st>>>(
-      x, x_dt, ldx, rows, static_cast<const uint8_t *>(w.codes), fp4_pitch(w.cols),
-      static_cast<const uint8_t *>(w.scales), fp4_chunks(w.cols, w.format), w.scale, w.rows, w.cols, out, dt, ld, sat);
-  return cudaGetLastError();
+  return 0;
+}
+
+template <int NH, int PARTS, int BLOCK>
+static cudaError_t v_launch(dim3 grid, size_t smem, cudaStream_t st, const GemvFp4Params &P) {
+  cudaError_t e = cudaFuncSetAttribute(gemv_fp4_kernel<NH, PARTS, BLOCK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       V_RING + V_SMEM_MAX);
+  if (e != cudaSuccess) return e;
+  PdlOff plain;  // a grid of this kind that may follow a persistent cluster kernel goes out in plain stream order
+  return launch_kernel(gemv_fp4_kernel<NH, PARTS, BLOCK>, grid, dim3(V_THREADS), smem, st, P.kparts, P);
 }
 
 int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const flux_cuda_fp4 &w, void *out, int dtype,
-                    long long ld_out, int num_sms, int *sat, cudaStream_t st) {
-  const long long steps = (static_cast<long long>(w.cols) + 1023) / 1024;
-  int s = rows == 1 ? 1 : rows == 2 ? 2 : 4;
-  while (s > 1 && s * steps * 4096 > V_SMEM_MAX) s /= 2;
-  const bool staged = s * steps * 4096 <= V_SMEM_MAX;
-  const size_t smem = staged ? static_cast<size_t>(s * steps * 4096) : 0;
-  const long long warps = fp4_row_tiles(w.rows) * 32;
-  const long long want = (warps + V_THREADS / 32 - 1) / (V_THREADS / 32);
-  dim3 grid(static_cast<unsigned>(want < num_sms ? want : num_sms), (rows + s - 1) / s);
+                    long long ld_out, int device, int *sat, cudaStream_t st) {
+  GemvFp4Params P = {};
+  P.x = x, P.ldx = ldx, P.rows = rows;
+  P.x_vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !(ldx * (x_dtype == FLUX_CUDA_F32 ? 4 : 2) & 15);
+  P.codes = static_cast<const uint8_t *>(w.codes), P.scales = static_cast<const uint8_t *>(w.scales);
+  P.pitch = fp4_pitch(w.cols), P.chunks = fp4_chunks(w.cols, w.format);
+  P.scale = w.scale, P.N = w.rows, P.K = w.cols;
+  P.steps = (w.cols + 255) / 256;
+  P.out = out, P.dt = dtype, P.ld = ld_out, P.sat = sat;
+  P.by = make_uint2((1u << 12) + (1u << 6), (1u << 8) + (1u << 2));
+  P.units = fp4_row_tiles(w.rows) * 4;
+  const int parts = x_dtype == FLUX_CUDA_BF16 ? 1 : x_dtype == FLUX_CUDA_F16 ? 2 : 3;
+  // Rows of x per block, and K in as many CTAs as it takes to fit them.
+  auto x_bytes = [&](int group, int kparts) {
+    return static_cast<long long>((P.steps + kparts - 1) / kparts) * 512 * parts * group;
+  };
+  const long long sums_room = 16384;
+  P.kparts = 1;
+  while (P.kparts < 8 && P.kparts * 2 <= P.steps && x_bytes(rows, P.kparts) > V_SMEM_MAX - sums_room * (1 + (rows > 4))) P.kparts *= 2;
+  P.group = rows;
+  while (P.group > 1 && x_bytes(P.group, P.kparts) + (2 * V_WARPS + 1) * 128LL * P.group > V_SMEM_MAX) P.group = (P.group + 1) / 2;
+  const int groups = (rows + P.group - 1) / P.group;
+  // Of the ways to split K further, as long as a warp gets a step, the one that ends first: clusters at once, and how evenly
+  // the units go into them.
+  auto held = [&](int kparts) {
+    const long long n = g_clusters[device][kparts == 1 ? 0 : kparts == 2 ? 1 : kparts == 4 ? 2 : 3] / groups;
+    return n < 1 ? 1 : n > P.units ? P.units : n;
+  };
+  auto longest = [&](int kparts) {  // steps that the busiest warp of a cluster does, and a little for every part
+    const long long n = held(kparts), rows_of_steps = (P.units + n - 1) / n * ((P.steps + kparts - 1) / kparts);
+    return static_cast<double>((rows_of_steps + V_WARPS - 1) / V_WARPS) + 0.5 * (kparts > 1);
+  };
+  int split = P.kparts;
+  for (int k = P.kparts * 2; k <= 8 && k <= P.steps; k *= 2)
+    if (longest(k) < longest(split)) split = k;
+  P.kparts = split;
+  P.part_steps = (P.steps + P.kparts - 1) / P.kparts;
+  long long clusters = held(P.kparts);
+  // the sums of a cluster's units next to x
+  const long long room = (V_SMEM_MAX - x_bytes(P.group, P.kparts)) / (128LL * P.group) - 2 * V_WARPS;
+  if (P.units > clusters * room) clusters = (P.units + room - 1) / room;
+  P.clusters = static_cast<int>(clusters);
+  const size_t smem = static_cast<size_t>(V_RING + x_bytes(P.group, P.kparts) +
+                                          ((P.units + clusters - 1) / clusters + 2 * V_WARPS) * 128 * P.group);
+  const dim3 grid(static_cast<unsigned>(clusters * P.kparts), groups);
   cudaError_t e;
-#define FX_V(S, ST)                                                                                                     \
-  e = w.format == 16 ? v_launch<S, 16, ST>(grid, smem, st, x, x_dtype, ldx, rows, w, out, dtype, ld_out, sat)             \
-                     : v_launch<S, 32, ST>(grid, smem, st, x, x_dtype, ldx, rows, w, out, dtype, ld_out, sat)
-  if (!staged) FX_V(1, false);
-  else if (s == 1) FX_V(1, true);
-  else if (s == 2) FX_V(2, true);
-  else FX_V(4, true);
+#define FX_V(NH, PARTS) e = w.format == 16 ? v_launch<NH, PARTS, 16>(grid, smem, st, P) : v_launch<NH, PARTS, 32>(grid, smem, st, P)
+  if (P.group <= 8) {
+    if (parts == 1) FX_V(1, 1);
+    else if (parts == 2) FX_V(1, 2);
+    else FX_V(1, 3);
+  } else {
+    if (parts == 1) FX_V(2, 1);
+    else if (parts == 2) FX_V(2, 2);
+    else FX_V(2, 3);
+  }
 #undef FX_V
   return e == cudaSuccess ? 0 : -8;
 }

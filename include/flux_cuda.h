@@ -463,7 +463,8 @@ int flux_cuda_qk_norm_rope(flux_cuda_ctx *ctx, void *qkv, long long ld, int q_co
  * scales: one byte per row r and block b, in tiles of 128 rows x 4 blocks of 512 bytes, tile (r / 128, b / 4) at
  *         ((r / 128) * ceil(blocks / 4) + b / 4) * 512, byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of it (the order
  *         the tensor cores take); rows and blocks past the end hold 0.
- * flux_cuda_fp4_quantize writes both, padding included; matrices from elsewhere must keep to it. Both 16-byte aligned;
+ * flux_cuda_fp4_quantize writes both, padding included; matrices from elsewhere must keep to it, and for the products hold
+ * no code * factor beyond the f32 range (MXFP4 factors above 2^125; the rows that do hold them come out unspecified). Both 16-byte aligned;
  * rows [128 i, ...) of a matrix are a matrix of their own (codes + 128 i * row bytes, scales + i * ceil(blocks / 4) * 512).
  * ---------------------------------------------------------------------------------------------- */
 #define FLUX_CUDA_NVFP4 16 /* blocks of 16 columns, factor e4m3 (at most 448; 0x7F is NaN) */
@@ -494,13 +495,14 @@ int flux_cuda_fp4_dequantize(flux_cuda_ctx *ctx, const flux_cuda_fp4 *q, void *o
  * flux_cuda_gemm_bf16's STORE and GATED_RES epilogues. x [M, K], w [N, K] of one format; any M, N >= 0, K >= 1. out of
  * `dtype` with row pitch ld_out; f32 sums, rounded once (f16 saturates and is counted). gate f32 [N] or NULL (1);
  * residual f32 [M, N] with row pitch ld_residual, or NULL (0); it may be `out` itself in f32 with the same pitch,
- * otherwise no output may overlap an input. A NaN factor makes the products of its row or column NaN.
+ * otherwise no output may overlap an input. Row pitches are below 2^30 elements. A NaN factor makes the products of its row or column NaN.
  */
 int flux_cuda_gemm_fp4(flux_cuda_ctx *ctx, const flux_cuda_fp4 *x, const flux_cuda_fp4 *w, void *out, int dtype,
                        long long ld_out, const float *gate, const float *residual, long long ld_residual);
 /*
  * The same product for 0 .. 16 rows of x that stay as they are (x_dtype, row pitch ldx): out[m, n] = sum_k x[m, k]
- * w[n, k], f32 sums. For single tokens and modulation vectors, where reading the weights is the whole cost.
+ * w[n, k], f32 sums of exact products. For single tokens and modulation vectors, where reading the weights is the whole
+ * cost. Up to 65536 columns.
  */
 int flux_cuda_gemv_fp4(flux_cuda_ctx *ctx, const void *x, int x_dtype, long long ldx, int rows, const flux_cuda_fp4 *w,
                        void *out, int dtype, long long ld_out);

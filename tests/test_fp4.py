@@ -86,13 +86,24 @@ def test_product_refusals(fx):
     _refused(fx, L.flux_cuda_gemm_fp4(None, x, w, GOOD, 0, 8, None, GOOD, 7), "row pitch")
     _refused(fx, L.flux_cuda_gemm_fp4(None, x, w, GOOD, 1, 8, None, GOOD, 8), "residual may be out itself")
     _refused(fx, L.flux_cuda_gemm_fp4(None, x, w, GOOD, 0, 8, None, GOOD, 9), "residual may be out itself")
-    big = _matrix(fx, rows=2 ** 31 - 1)
-    _refused(fx, L.flux_cuda_gemm_fp4(None, big, big, GOOD, 0, 2 ** 31, None, None, 0), "too many")
+    big = _matrix(fx, rows=2 ** 29)
+    _refused(fx, L.flux_cuda_gemm_fp4(None, big, big, GOOD, 0, 2 ** 29, None, None, 0), "too many")
 
 
 @pytest.mark.parametrize("rows", [-1, 17, 1000])
 def test_few_row_product_takes_few_rows(fx, rows):
     _refused(fx, fx.lib().flux_cuda_gemv_fp4(None, GOOD, 0, 64, rows, _matrix(fx), GOOD, 0, 64), "0 to 16 rows")
+
+
+def test_few_row_product_takes_rows_of_a_length(fx):
+    w = _matrix(fx, cols=65537)
+    _refused(fx, fx.lib().flux_cuda_gemv_fp4(None, GOOD, 0, 65537, 1, w, GOOD, 0, 64), "65536 columns")
+
+
+def test_product_pitches(fx):
+    L, x, w = fx.lib(), _matrix(fx), _matrix(fx, rows=8)
+    _refused(fx, L.flux_cuda_gemm_fp4(None, x, w, GOOD, 0, 2 ** 30, None, None, 0), "row pitch")
+    _refused(fx, L.flux_cuda_gemm_fp4(None, x, w, GOOD, 0, 8, None, ctypes.c_void_p(8192), 2 ** 30), "row pitch")
 
 
 def test_a_null_context_is_refused_last(fx):

@@ -317,6 +317,14 @@ def test_product_of_a_row_slice(fx, ctx):
     assert (np.abs(out.double().cpu().numpy() - want) <= _product_tolerance(xv, wv[128:], want, "f32", None, None)).all()
 
 
+def _few_row_tolerance(mag, K, xname):
+    """f32 sums of exact products: an instruction adds the products of 16 columns and one bf16 part of x to the accumulator,
+    at most a truncation of the running sum and one of the aligned products, 2^-23 of the sum of magnitudes each; then at
+    most 64 partial sums, and the scale (a rounding, and one for the tests' own use of it)."""
+    parts = {"bf16": 1, "f16": 2, "f32": 3}[xname]
+    return mag * (2 * parts * -(-K // 16) + 64 + 2) * 2.0 ** -23
+
+
 @pytest.mark.parametrize("fmt", [16, 32])
 @pytest.mark.parametrize("xname,out", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f32", "bf16")])
 @pytest.mark.parametrize("M,N,K,pad", [(1, 1, 1, 0), (1, 300, 2560, 0), (2, 129, 1025, 3), (3, 128, 31, 1), (4, 260, 96, 0),
@@ -332,17 +340,15 @@ def test_few_row_product(fx, ctx, M, N, K, pad, xname, out, fmt):
     wv = wv / 0.7 * float(np.float32(0.7))
     want = x @ wv.T
     mag = np.abs(x) @ np.abs(wv).T
-    # f32 sums: a lane adds at most 32 products per 1024 columns one after the other, 16 of them before the factor, then
-    # five additions over the warp and the scale; a rounding of at most the sum of magnitudes each
-    tol = mag * (32 * -(-K // 1024) + 16 + 8) * 2.0 ** -24 + HALF_STEP[out] * np.abs(want) + TINY[out]
+    tol = _few_row_tolerance(mag, K, xname) + HALF_STEP[out] * np.abs(want) + TINY[out]
     have = got.double().cpu().numpy()
     assert (np.abs(have[:M, :N] - want) <= tol).all()
     assert (have[M:] == 7).all() and (have[:, N:] == 7).all()
 
 
-@pytest.mark.parametrize("M,K", [(1, 60000), (3, 20000)])
+@pytest.mark.parametrize("M,K", [(1, 60000), (3, 20000), (16, 30000), (1, 65536), (5, 65536)])
 def test_few_row_product_of_long_rows(fx, ctx, M, K):
-    """Rows of x that do not fit shared memory, or fit it only one at a time."""
+    """Rows of x that fit shared memory only in parts, or not all at once."""
     rng = np.random.default_rng(K)
     w, wv = _random_matrix(fx, rng, 40, K, 16)
     dev, x = _plain(rng.standard_normal((M, K)), "f32", K)
@@ -351,8 +357,78 @@ def test_few_row_product_of_long_rows(fx, ctx, M, K):
     ctx.gemv_fp4(dev.data_ptr(), fx.F32, K, M, w.h, out.data_ptr(), fx.F32, 40)
     ctx.sync()
     want = x @ wv.T
-    tol = (np.abs(x) @ np.abs(wv).T) * (32 * -(-K // 1024) + 24) * 2.0 ** -24 + 2.0 ** -24 * np.abs(want)
+    tol = _few_row_tolerance(np.abs(x) @ np.abs(wv).T, K, "f32") + 2.0 ** -24 * np.abs(want)
     assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("N,K", [(2560, 9728), (19000, 300), (9728, 1000), (128, 128)])
+def test_few_row_product_of_many_columns(fx, ctx, N, K):
+    """Several rounds of weight rows per block, and K split among warps and CTAs."""
+    rng = np.random.default_rng(N)
+    for M, name in ((1, "bf16"), (4, "f32"), (16, "f16")):
+        w, wv = _random_matrix(fx, rng, N, K, 32 if M == 4 else 16, std=0.1)
+        dev, x = _plain(rng.standard_normal((M, K)), name, K)
+        out = torch.zeros(M, N, device="cuda")
+        torch.cuda.synchronize()
+        ctx.gemv_fp4(dev.data_ptr(), _dt(fx, name), K, M, w.h, out.data_ptr(), fx.F32, N)
+        ctx.sync()
+        want = x @ wv.T
+        tol = _few_row_tolerance(np.abs(x) @ np.abs(wv).T, K, name) + 2.0 ** -24 * np.abs(want)
+        assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+def test_few_row_product_with_every_factor(fx, ctx, fmt):
+    """Every finite factor with every code, against x that picks out one column: exact products, so exact results (where
+    they are normal f32 values). Factors of NaN give NaN in their row."""
+    code = np.tile(np.arange(16), (256, fmt // 16))
+    byte = np.arange(256).astype(np.uint8)[:, None]
+    if fmt == 16:
+        byte &= 127
+    w = Matrix(fx, 256, fmt, fmt, 1.0, ref.pack(code, byte))
+    wv = ref.values(code, byte, fmt)
+    for name in ("f32", "f16", "bf16"):
+        for first in range(0, fmt, 16):
+            x = np.zeros((16, fmt))
+            x[np.arange(16), first + np.arange(16)] = {"f32": 1 + 2.0 ** -23, "f16": 1 + 2.0 ** -10, "bf16": 1 + 2.0 ** -7}[name]
+            dev, xv = _plain(x, name, fmt)
+            out = torch.zeros(16, 256, device="cuda")
+            torch.cuda.synchronize()
+            ctx.gemv_fp4(dev.data_ptr(), _dt(fx, name), fmt, 16, w.h, out.data_ptr(), fx.F32, 256)
+            ctx.sync()
+            with np.errstate(over="ignore"):
+                want = np.stack([(xv[i, first + i] * wv[:, first + i]) for i in range(16)])
+            got = out.double().cpu().numpy()
+            # rows of w that hold values beyond the f32 range (factors above 2^125) are left to the formats
+            inside = np.isnan(wv).any(1) | (np.abs(wv).max(1) < 3.4e38)
+            assert inside.sum() >= 254 - 2
+            assert (np.isnan(got) == np.isnan(want))[:, inside].all()
+            # parts of x times a weight are exact; adding up to three of them rounds twice
+            fine = inside & np.isfinite(want) & (np.abs(want) < 3e38) & ((np.abs(want) > 2.0 ** -100) | (want == 0))
+            assert (np.abs(got - want)[fine] <= 2 * 2.0 ** -23 * np.abs(want)[fine]).all()
+
+
+def test_few_row_product_of_extreme_rows(fx, ctx):
+    """Rows of x with infinities, NaN and values at both ends of the f32 range stay rows of their own; a huge value at a
+    weight of zero does not cost its neighbours their digits."""
+    code = np.zeros((40, 64), np.int64)
+    code[:, 1:] = 2  # 1.0, but for column 0
+    w = Matrix(fx, 40, 64, 16, 1.0, ref.pack(code, np.full((40, 4), 0x38, np.uint8)))  # factors of 1
+    x = np.zeros((6, 64))
+    x[0, 0], x[0, 1] = 3e38, 1e-30
+    x[1, 1] = float(np.finfo(np.float32).max)
+    x[2, 5], x[3, 6] = np.inf, np.nan
+    x[4, 0] = np.inf  # times zero
+    x[5, 3] = 1.5
+    dev, xv = _plain(x, "f32", 64)
+    out = torch.zeros(6, 40, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemv_fp4(dev.data_ptr(), fx.F32, 64, 6, w.h, out.data_ptr(), fx.F32, 40)
+    ctx.sync()
+    got = out.double().cpu().numpy()
+    assert (np.abs(got[0] - xv[0, 1]) <= 2.0 ** -22 * 1e-30).all()
+    assert (np.abs(got[1] / xv[1, 1] - 1) <= 2.0 ** -22).all()
+    assert (got[2] == np.inf).all() and np.isnan(got[3]).all() and np.isnan(got[4]).all() and (got[5] == 1.5).all()
 
 
 def test_nothing_to_do(fx, ctx):
