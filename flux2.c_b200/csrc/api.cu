@@ -112,7 +112,7 @@ int flux_cuda_ctx_create(int device, flux_cuda_ctx **out) {
   if (const char *e = getenv("FLUX_CUDA_BF16")) c->f16 = atoi(e) == 0;
   if (const char *e = getenv("FLUX_CUDA_ATTN")) c->attn_version = atoi(e) == 3 ? 3 : 2;
   if (gemm_init() != 0 || gemm2_init() != 0 || attn2_init() != 0 || attn3_init() != 0 || elementwise_init() != 0 ||
-      conv_init() != 0 || fp4_gemm_init() != 0 || fp4_gemv_init(device) != 0) {
+      conv_init() != 0 || fp4_gemm_init(device) != 0 || fp4_gemv_init(device) != 0) {
     set_error("could not resolve cuTensorMapEncodeTiled / configure shared memory");
     flux_cuda_ctx_destroy(c);
     return FLUX_CUDA_ERR_CUDA;

@@ -35,11 +35,12 @@ struct Fp4GemmArgs {
 // All return 0, or -8 for a failed launch / -4 for a tensor map the driver refuses.
 int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda_fp4 &q, cudaStream_t st);
 int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long long ld, int *sat, cudaStream_t st);
-int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st);
+int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cudaStream_t st);
 int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const flux_cuda_fp4 &w, void *out, int dtype,
                     long long ld_out, int device, int *sat, cudaStream_t st);
-int fp4_gemm_init();  // opts the product kernels into large shared memory
-int fp4_gemv_init(int device);  // counts the clusters that the current device holds
+// For the current device, once per context: large shared memory, and how many clusters the device holds at once.
+int fp4_gemm_init(int device);
+int fp4_gemv_init(int device);
 
 static constexpr int FP4_GEMV_MAX_ROWS = 16, FP4_GEMV_MAX_COLS = 65536;  // what eight SMs' shared memory holds of x
 

@@ -116,7 +116,7 @@ int flux_cuda_gemm_fp4(flux_cuda_ctx *ctx, const flux_cuda_fp4 *x, const flux_cu
   if (x->rows == 0 || w->rows == 0) return FLUX_CUDA_OK;
   OnDevice on(ctx->device);
   Fp4GemmArgs a = {*x, *w, out, dtype, ld_out, gate, residual, ld_residual};
-  return finish(op, launch_gemm_fp4(a, ctx->num_sms, ctx->err_dev, ctx->stream));
+  return finish(op, launch_gemm_fp4(a, ctx->device, ctx->num_sms, ctx->err_dev, ctx->stream));
 }
 
 int flux_cuda_gemv_fp4(flux_cuda_ctx *ctx, const void *x, int x_dtype, long long ldx, int rows, const flux_cuda_fp4 *w,

@@ -161,6 +161,7 @@ __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m
   for (int i = 0; i < 4; ++i) g[i] = gate && n + i < N ? alpha * gate[n + i] : alpha;
   for (; m < m_end; m += 4 * R) {
     float4 v[SP][R];
+    float y[R][4];  // the residual, all of it requested before anything is stored (it may be `out`)
 #pragma unroll
     for (int s = 0; s < SP; ++s) {
       if (s >= splits) break;
@@ -169,22 +170,28 @@ __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m
       for (int j = 0; j < R; ++j) v[s][j] = ld_cluster_f32x4(from + (m + 4 * j < m_end ? m + 4 * j : m) * F_BN * 4);
     }
 #pragma unroll
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        y[j][i] = res && m + 4 * j < m_end && n + i < N
+                      ? __ldcg(reinterpret_cast<const float *>(res + (m + 4 * j) * res_pitch + i * 4))
+                      : 0.f;
+#pragma unroll
     for (int j = 0; j < R; ++j) {
       float4 a = v[0][j];
 #pragma unroll
       for (int s = 1; s < SP; ++s)
         if (s < splits) a.x += v[s][j].x, a.y += v[s][j].y, a.z += v[s][j].z, a.w += v[s][j].w;
-      const int row = m + 4 * j;
-      if (row >= m_end) continue;
-      const float e[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (n + i >= N) continue;
-        float y = g[i] * e[i];
-        if (res) y = fmaf(g[i], e[i], __ldcg(reinterpret_cast<const float *>(res + row * res_pitch + i * 4)));
-        fp4_store<DT>(out + row * pitch, i, y, mx);
-      }
+      y[j][0] = fmaf(g[0], a.x, y[j][0]);
+      y[j][1] = fmaf(g[1], a.y, y[j][1]);
+      y[j][2] = fmaf(g[2], a.z, y[j][2]);
+      y[j][3] = fmaf(g[3], a.w, y[j][3]);
     }
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (m + 4 * j < m_end && n + i < N) fp4_store<DT>(out + (m + 4 * j) * pitch, i, y[j][i], mx);
   }
 }
 
@@ -575,7 +582,12 @@ static cudaError_t opt_in_pair() {
   return e;
 }
 
-int fp4_gemm_init() {
+// Clusters of 1 to 8 CTAs of the 128-row kernel (two per SM, as the smaller ones) that a device holds at once: the GPCs'
+// numbers of SMs are no multiples of most sizes, so they are fewer than the SMs make.
+static int g_fp4_clusters[64][9];
+
+int fp4_gemm_init(int device) {
+  if (device < 0 || device >= 64) return -1;
   if (!g_encode4) {
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult qres;
@@ -587,7 +599,24 @@ int fp4_gemm_init() {
                   opt_in<32, 32>() == cudaSuccess && opt_in<64, 16>() == cudaSuccess && opt_in<64, 32>() == cudaSuccess &&
                   opt_in<128, 16>() == cudaSuccess && opt_in<128, 32>() == cudaSuccess &&
                   opt_in_pair<16>() == cudaSuccess && opt_in_pair<32>() == cudaSuccess;
-  return ok ? 0 : -2;
+  if (!ok) return -2;
+  for (int s = 1; s <= 8; ++s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024 / s * s);
+    cfg.blockDim = dim3(F_THREADS);
+    cfg.dynamicSmemBytes = FCfg<128, 16>::SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = s;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&g_fp4_clusters[device][s], gemm_fp4_kernel<128, 16, FLUX_CUDA_BF16>, &cfg) !=
+            cudaSuccess ||
+        g_fp4_clusters[device][s] < 1)
+      return -2;
+  }
+  return 0;
 }
 
 // The codes of a matrix as bytes, in boxes of box_rows x 128.
@@ -637,7 +666,7 @@ static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype,
 // measured on a B200 (148 SMs) and matter only relative to one another.
 //   One CTA per tile: 2.5 to start and stop, a k-slice 0.33 while the ring's latency bounds it (0.45 with the three stages
 //   of the 128-row tile) and its bytes over 12 TB/s of L2 when many CTAs run (a pitch off the 128-byte lines costs 1.6
-//   times as much), two CTAs per SM and wave; a split adds a cluster launch and the exchange of the partial tile.
+//   times as much), as many clusters at once as the device holds; a split adds a cluster launch and the exchange of the partial tile.
 //   Pairs: a k-slice 0.35, an epilogue of 2 that the next tile's products hide.
 // Measured at 1024 x 1024 x 1024: 64 rows 4.8, 128 rows 5.8, pairs 7.0; 512 x 2560 x 9728: 128 rows 20.8 alone, 16.2 split
 // three ways, pairs 19.2; 1 x 2560 x 9728: 16.0 alone, 6.1 split eight ways; 128 x 2560 x 2560: 64 rows 6.8 alone, 7.6 split
@@ -645,7 +674,7 @@ static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype,
 struct Fp4Choice {
   int bm, splits;  // bm 256: pairs
 };
-static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_sms) {
+static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_sms, const int *clusters) {
   const long long tn = (N + F_BN - 1) / F_BN;
   Fp4Choice best = {128, 1};
   double least = 1e30;
@@ -653,8 +682,8 @@ static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_s
     if (bm < 64 && M > bm) continue;  // a tile starts on half a factor tile at the least
     const long long tiles = tn * ((M + bm - 1) / bm);
     for (int s = 1; s <= 8 && s <= slices; ++s) {
-      const long long ctas = tiles * s, slots = 2LL * num_sms;
-      const double active = ctas < slots ? ctas : slots, waves = (ctas + slots - 1) / slots;
+      const long long at_once = clusters[s];
+      const double active = static_cast<double>(tiles < at_once ? tiles : at_once) * s, waves = (tiles + at_once - 1) / at_once;
       const double latency = bm == 128 ? 0.45 : 0.33;
       const double bytes = active * (F_W_BYTES + bm * F_KB + 4096) / 12e6 * (pitch % 128 ? 1.6 : 1.0);
       const double t = 2.5 + waves * ((slices + s - 1) / s) * (latency > bytes ? latency : bytes) +
@@ -671,12 +700,12 @@ static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_s
   return best;
 }
 
-int launch_gemm_fp4(const Fp4GemmArgs &a, int num_sms, int *err, cudaStream_t st) {
+int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cudaStream_t st) {
   Fp4GemmParams P;
   memset(&P, 0, sizeof(P));
   const int M = a.x.rows, N = a.w.rows, block = a.x.format;
   const int slices = static_cast<int>((static_cast<long long>(a.x.cols) + 255) / 256);
-  const Fp4Choice choice = fp4_choose(M, N, slices, fp4_pitch(a.x.cols), num_sms);
+  const Fp4Choice choice = fp4_choose(M, N, slices, fp4_pitch(a.x.cols), num_sms, g_fp4_clusters[device]);
   const int bm = choice.bm;
   const bool pair = bm == 256;
   const uint32_t chunks = 256 / (4 * block);
