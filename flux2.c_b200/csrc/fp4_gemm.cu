@@ -112,18 +112,26 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   return v;
 }
 
-// Epilogue of 16 output rows of this thread's column n, starting at `out` (and `res`): a = alpha * gate. Each row's address
-// is one multiply-add of its own (row pitches are 32 bits, checked on the host), the residual is fetched for all rows
-// before the first store, and whole blocks carry no predicates: one warp per scheduler has nothing to hide a chain of
-// 64-bit additions or a branch behind. Checked and addressed row by row a store cost 150 cycles, along a chain 32.
-template <int DT>
-__device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], int rows, uint8_t *out, uint32_t pitch, const uint8_t *res,
-                                         uint32_t res_pitch, float a, float &mx) {
-  float v[16];
-  if (res) {
+// The residual of 16 output rows of this thread's column, requested well before fp4_emit wants it (a load takes most of a
+// microsecond, and the stores in between keep the compiler from moving it). Only where there is one.
+__device__ __forceinline__ void fp4_residual(float (&v)[16], int rows, const uint8_t *res, uint32_t res_pitch) {
+  if (rows >= 16) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __ldcg(reinterpret_cast<const float *>(res + static_cast<uint64_t>(res_pitch) * j));
+  } else {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       v[j] = j < rows ? __ldcg(reinterpret_cast<const float *>(res + static_cast<uint64_t>(res_pitch) * j)) : 0.f;
+  }
+}
+// Epilogue of 16 output rows of this thread's column n, starting at `out`: a = alpha * gate, v the residual if any. Each row's
+// address is one multiply-add of its own (row pitches are 32 bits, checked on the host), and whole blocks carry no
+// predicates: one warp per scheduler has nothing to hide a chain of 64-bit additions or a branch behind. Checked and
+// addressed row by row a store cost 150 cycles, along a chain 32.
+template <int DT>
+__device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], float (&v)[16], bool residual, int rows, uint8_t *out,
+                                         uint32_t pitch, float a, float &mx) {
+  if (residual) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = fmaf(a, __uint_as_float(r[j]), v[j]);
   } else {
@@ -306,9 +314,6 @@ __global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_con
   } else {
     const int q = warp & 3;  // the lane group of TMEM this warp may read
     const int nl = q * 32 + lane, n = n0 + nl;
-    const bool ok = mbar_wait_warp(tfull, 0, abort_flag);
-    if (!ok && lane == 0) fail(KERR_WAIT_TMEM_FULL);
-    tc_fence_after_sync();
     const int live = P.M - m0 < BM ? P.M - m0 : BM;
     const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
     float mx = 0.f;
@@ -316,6 +321,12 @@ __global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_con
     uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * FP4_SIZE<DT>;
     const uint8_t *res = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + n * 4LL : nullptr;
     constexpr int STEP = 16;
+    const bool direct = P.splits == 1 && n < P.N;
+    float v[16];
+    if (direct && res) fp4_residual(v, live, res, P.res_pitch);
+    const bool ok = mbar_wait_warp(tfull, 0, abort_flag);
+    if (!ok && lane == 0) fail(KERR_WAIT_TMEM_FULL);
+    tc_fence_after_sync();
     float *part = reinterpret_cast<float *>(smem);  // every MMA has read its operands by now
     if (ok) {
 #pragma unroll 1  // see the pair kernel
@@ -328,8 +339,14 @@ __global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_con
         if (P.splits > 1) {
 #pragma unroll
           for (int j = 0; j < STEP; ++j) part[(c + j) * F_BN + nl] = __uint_as_float(r[j]);
-        } else if (n < P.N) {
-          fp4_emit<DT>(r, live - c, out + c * pitch, P.pitch, res ? res + c * res_pitch : res, P.res_pitch, a, mx);
+        } else if (direct) {
+          float next[16];
+          if (res) fp4_residual(next, live - c - STEP, res + (c + STEP) * res_pitch, P.res_pitch);
+          fp4_emit<DT>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, mx);
+          if (res) {
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) v[j] = next[j];
+          }
         }
       }
     }
@@ -501,11 +518,6 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
     uint32_t t = 0;
     for (int tile = pair; tile < P.tiles; tile += num_pairs, ++t) {
       const int m0 = (tile % P.tiles_m) * 256, n = (tile / P.tiles_m) * 256 + static_cast<int>(rank) * 128 + q * 32 + lane;
-      if (!mbar_wait_warp(&tfull[t & 1], (t >> 1) & 1, abort_flag)) {
-        if (lane == 0) fail(KERR_WAIT_TMEM_FULL);
-        break;
-      }
-      tc_fence_after_sync();
       const int live = n < P.N ? (P.M - m0 < 256 ? P.M - m0 : 256) : 0;
       const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
       const uint32_t acc = tmem + (t & 1) * C::ACC1 + (static_cast<uint32_t>(q * 32) << 16);
@@ -519,10 +531,21 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
       // 40 KB of straight-line code ran at the speed of instruction fetches and took the issuer's loop out of the cache.
       const int shared = (t & 1) ? 0 : C::ACC1;
       uint32_t r0[16], r1[16];
+      float v0[16], v1[16];
       auto column = [&](int i) { return (shared + 16 * (2 * i + half)) & 255; };
-      auto finish = [&](const uint32_t (&r)[16], int c) {
-        fp4_emit<DT>(r, live - c, out + c * pitch, P.pitch, res ? res + c * res_pitch : res, P.res_pitch, a, mx);
+      auto finish = [&](const uint32_t (&r)[16], float (&v)[16], int c) {
+        fp4_emit<DT>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, mx);
       };
+      auto fetch = [&](float (&v)[16], int c) {
+        if (res) fp4_residual(v, live - c, res + c * res_pitch, P.res_pitch);
+      };
+      fetch(v0, column(0));  // while the tile is still being computed
+      fetch(v1, column(1));
+      if (!mbar_wait_warp(&tfull[t & 1], (t >> 1) & 1, abort_flag)) {
+        if (lane == 0) fail(KERR_WAIT_TMEM_FULL);
+        break;
+      }
+      tc_fence_after_sync();
       tc_ld_32x16(acc + column(0), r0);
       tc_ld_32x16(acc + column(1), r1);
       tc_wait_ld();
@@ -531,10 +554,16 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
       if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(drained), 0));
 #pragma unroll 1
       for (int i = 0; i < 8; i += 2) {
-        finish(r0, column(i));
-        if (i < 6) tc_ld_32x16(acc + column(i + 2), r0);
-        finish(r1, column(i + 1));
-        if (i < 6) tc_ld_32x16(acc + column(i + 3), r1);
+        finish(r0, v0, column(i));
+        if (i < 6) {
+          tc_ld_32x16(acc + column(i + 2), r0);
+          fetch(v0, column(i + 2));
+        }
+        finish(r1, v1, column(i + 1));
+        if (i < 6) {
+          tc_ld_32x16(acc + column(i + 3), r1);
+          fetch(v1, column(i + 3));
+        }
         tc_wait_ld();
       }
     }
