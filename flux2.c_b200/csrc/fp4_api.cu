@@ -55,6 +55,9 @@ int check_plain(const char *op, const char *name, const void *p, int dtype, long
   return FLUX_CUDA_ERR_ARG;
 }
 
+// Quantising and back take blocks of 32 rows x 256 columns.
+bool too_large(const flux_cuda_fp4 &q) { return fp4_row_tiles(q.rows) * 4 * ((q.cols + 255LL) / 256) > 0x7FFFFFFF; }
+
 int finish(const char *op, int rc) {
   if (rc == 0) return FLUX_CUDA_OK;
   set_error("%s: %s: %s", op, rc == -4 ? "tensor map refused" : "launch failed", cudaGetErrorString(cudaGetLastError()));
@@ -80,6 +83,7 @@ int flux_cuda_fp4_quantize(flux_cuda_ctx *ctx, const void *x, int dtype, long lo
   int rc = check_matrix(op, "q", q);
   if (rc || (rc = check_plain(op, "x", x, dtype, ldx, q->rows, q->cols))) return rc;
   int e;
+  if (too_large(*q)) return refuse(op, "q is too large for one launch");
   if (frexpf(q->scale, &e) != 0.5f || e < -99 || e > 101) return refuse(op, "q's scale is not a power of two in 2^-100 .. 2^100");
   if (!ctx) return refuse(op, "null context");
   if (q->rows == 0) return FLUX_CUDA_OK;
@@ -91,6 +95,7 @@ int flux_cuda_fp4_dequantize(flux_cuda_ctx *ctx, const flux_cuda_fp4 *q, void *o
   const char *op = "fp4_dequantize";
   int rc = check_matrix(op, "q", q);
   if (rc || (rc = check_plain(op, "out", out, dtype, ld, q->rows, q->cols))) return rc;
+  if (too_large(*q)) return refuse(op, "q is too large for one launch");
   if (!ctx) return refuse(op, "null context");
   if (q->rows == 0) return FLUX_CUDA_OK;
   OnDevice on(ctx->device);

@@ -640,10 +640,9 @@ int fp4_gemm_init(int device) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&g_fp4_clusters[device][s], gemm_fp4_kernel<128, 16, FLUX_CUDA_BF16>, &cfg) !=
-            cudaSuccess ||
-        g_fp4_clusters[device][s] < 1)
-      return -2;
+    int n = 0;  // none: this size is not used
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_fp4_kernel<128, 16, FLUX_CUDA_BF16>, &cfg) != cudaSuccess) cudaGetLastError();
+    g_fp4_clusters[device][s] = s == 1 && n < 1 ? 1 : n;
   }
   return 0;
 }
@@ -712,6 +711,7 @@ static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_s
     const long long tiles = tn * ((M + bm - 1) / bm);
     for (int s = 1; s <= 8 && s <= slices; ++s) {
       const long long at_once = clusters[s];
+      if (at_once < 1) continue;
       const double active = static_cast<double>(tiles < at_once ? tiles : at_once) * s, waves = (tiles + at_once - 1) / at_once;
       const double latency = bm == 128 ? 0.45 : 0.33;
       const double bytes = active * (F_W_BYTES + bm * F_KB + 4096) / 12e6 * (pitch % 128 ? 1.6 : 1.0);

@@ -363,14 +363,20 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
 // Clusters of 1, 2, 4 and 8 blocks that a device holds at once, one block per SM (the GPCs' numbers of SMs are no multiples of
 // eight, so they are fewer than the SMs make).
 static int g_clusters[64][4];
+template <int NH, int PARTS>
+static bool v_opt_in() {
+  return cudaFuncSetAttribute(gemv_fp4_kernel<NH, PARTS, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              V_RING + V_SMEM_MAX) == cudaSuccess &&
+         cudaFuncSetAttribute(gemv_fp4_kernel<NH, PARTS, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              V_RING + V_SMEM_MAX) == cudaSuccess;
+}
 int fp4_gemv_init(int device) {
   if (device < 0 || device >= 64) return -1;
-  auto *kernel = gemv_fp4_kernel<1, 1, 16>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, V_RING + V_SMEM_MAX) != cudaSuccess) return -2;
+  if (!v_opt_in<1, 1>() || !v_opt_in<1, 2>() || !v_opt_in<1, 3>() || !v_opt_in<2, 1>() || !v_opt_in<2, 2>() || !v_opt_in<2, 3>())
+    return -2;
   for (int i = 0; i < 4; ++i) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(148 << i);
-    cfg.gridDim.x = (cfg.gridDim.x >> i) << i;
+    cfg.gridDim = dim3(128 << i);
     cfg.blockDim = dim3(V_THREADS);
     cfg.dynamicSmemBytes = V_RING + V_SMEM_MAX;
     cudaLaunchAttribute attr[1];
@@ -379,8 +385,8 @@ int fp4_gemv_init(int device) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return -2;
+    int n = 0;  // none: this size is not used unless x needs it
+    if (cudaOccupancyMaxActiveClusters(&n, gemv_fp4_kernel<1, 1, 16>, &cfg) != cudaSuccess) cudaGetLastError();
     g_clusters[device][i] = n;
   }
   return 0;
@@ -388,9 +394,6 @@ int fp4_gemv_init(int device) {
 
 template <int NH, int PARTS, int BLOCK>
 static cudaError_t v_launch(dim3 grid, size_t smem, cudaStream_t st, const GemvFp4Params &P) {
-  cudaError_t e = cudaFuncSetAttribute(gemv_fp4_kernel<NH, PARTS, BLOCK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       V_RING + V_SMEM_MAX);
-  if (e != cudaSuccess) return e;
   PdlOff plain;  // a grid of this kind that may follow a persistent cluster kernel goes out in plain stream order
   return launch_kernel(gemv_fp4_kernel<NH, PARTS, BLOCK>, grid, dim3(V_THREADS), smem, st, P.kparts, P);
 }
@@ -429,8 +432,8 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
     return static_cast<double>((rows_of_steps + V_WARPS - 1) / V_WARPS) + 0.5 * (kparts > 1);
   };
   int split = P.kparts;
-  for (int k = P.kparts * 2; k <= 8 && k <= P.steps; k *= 2)
-    if (longest(k) < longest(split)) split = k;
+  for (int k = P.kparts * 2, i = P.kparts == 1 ? 1 : P.kparts == 2 ? 2 : 3; k <= 8 && k <= P.steps; k *= 2, ++i)
+    if (g_clusters[device][i] > 0 && longest(k) < longest(split)) split = k;
   P.kparts = split;
   P.part_steps = (P.steps + P.kparts - 1) / P.kparts;
   long long clusters = held(P.kparts);

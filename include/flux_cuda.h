@@ -467,7 +467,7 @@ int flux_cuda_qk_norm_rope(flux_cuda_ctx *ctx, void *qkv, long long ld, int q_co
  * no code * factor beyond the f32 range (MXFP4 factors above 2^125; the rows that do hold them come out unspecified). Both 16-byte aligned;
  * rows [128 i, ...) of a matrix are a matrix of their own (codes + 128 i * row bytes, scales + i * ceil(blocks / 4) * 512).
  * ---------------------------------------------------------------------------------------------- */
-#define FLUX_CUDA_NVFP4 16 /* blocks of 16 columns, factor e4m3 (at most 448; 0x7F is NaN) */
+#define FLUX_CUDA_NVFP4 16 /* blocks of 16 columns, factor e4m3 without a sign (bytes 0 .. 0x7E, at most 448; 0x7F is NaN) */
 #define FLUX_CUDA_MXFP4 32 /* blocks of 32 columns, factor 2^(byte - 127) (0xFF is NaN) */
 
 typedef struct flux_cuda_fp4 {

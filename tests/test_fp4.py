@@ -76,6 +76,12 @@ def test_quantize_wants_a_power_of_two(fx, scale):
     _refused(fx, fx.lib().flux_cuda_fp4_quantize(None, GOOD, 0, 64, _matrix(fx, scale=scale)), "power of two")
 
 
+def test_matrices_beyond_a_launch_are_refused(fx):
+    L, q = fx.lib(), _matrix(fx, rows=2 ** 31 - 1, cols=2 ** 20)
+    _refused(fx, L.flux_cuda_fp4_quantize(None, GOOD, 0, 2 ** 20, q), "too large")
+    _refused(fx, L.flux_cuda_fp4_dequantize(None, q, GOOD, 0, 2 ** 20), "too large")
+
+
 def test_product_refusals(fx):
     L = fx.lib()
     x, w = _matrix(fx), _matrix(fx, rows=8)
