@@ -509,6 +509,135 @@ def test_a_feed_forward_block(fx, ctx, M, fmt):
         assert torch.equal(res, first)
 
 
+def test_every_operator_captured_and_replayed(fx, ctx):
+    """Two graphs of the same calls on different data share nothing; replays give the bits of the eager calls."""
+    rng = np.random.default_rng(30)
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    jobs = []
+    for seed in (1, 2):
+        x = torch.from_numpy(rng.standard_normal((9, 4096)).astype(np.float32)).cuda()
+        w, _ = _random_matrix(fx, rng, 500, 4096, 16)
+        q = Matrix(fx, 9, 4096, 16)
+        outs = [torch.zeros(9, 4096, device="cuda"), torch.zeros(9, 500, device="cuda"), torch.zeros(9, 500, device="cuda")]
+
+        def run(x=x, w=w, q=q, outs=outs):
+            ctx.fp4_quantize(x.data_ptr(), fx.F32, 4096, q.h)
+            ctx.fp4_dequantize(q.h, outs[0].data_ptr(), fx.F32, 4096)
+            ctx.gemm_fp4(q.h, w.h, outs[1].data_ptr(), fx.F32, 500)
+            ctx.gemv_fp4(x.data_ptr(), fx.F32, 4096, 9, w.h, outs[2].data_ptr(), fx.F32, 500)
+
+        torch.cuda.synchronize()
+        run()
+        ctx.sync()
+        eager = [o.clone() for o in outs]
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            run()
+        jobs.append((graph, outs, eager, q, x, w))
+    for _ in range(3):
+        for _, outs, _, _, _, _ in jobs:
+            for o in outs:
+                o.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for graph, _, _, _, _, _ in jobs:
+                graph.replay()
+        ctx.sync()
+        for _, outs, eager, _, _, _ in jobs:
+            assert all(torch.equal(o, e) for o, e in zip(outs, eager))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 2560, 9728), (5, 700, 20000), (64, 300, 9000), (130, 1000, 5000), (1100, 2300, 2000)])
+def test_products_repeat_bit_for_bit(fx, ctx, M, N, K):
+    """Split sums are added in a fixed order."""
+    rng = np.random.default_rng(M + K)
+    x, _ = _random_matrix(fx, rng, M, K, 16)
+    w, _ = _random_matrix(fx, rng, N, K, 16)
+    xs = torch.from_numpy(rng.standard_normal((min(M, 16), K)).astype(np.float32)).cuda()
+    first = None
+    for _ in range(4):
+        a, b = torch.zeros(M, N, device="cuda"), torch.zeros(min(M, 16), N, device="cuda")
+        torch.cuda.synchronize()
+        ctx.gemm_fp4(x.h, w.h, a.data_ptr(), fx.F32, N)
+        ctx.gemv_fp4(xs.data_ptr(), fx.F32, K, min(M, 16), w.h, b.data_ptr(), fx.F32, N)
+        ctx.sync()
+        assert first is None or (torch.equal(a, first[0]) and torch.equal(b, first[1]))
+        first = (a, b)
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+def test_offsets_beyond_32_bits(fx, ctx, fmt):
+    """The last rows of matrices of more than 2^32 bytes and 2^31 elements come out as they do alone."""
+    rows, cols, tail, K = 300003, 8192, 259, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[:-tail] = 1.0
+    x[-tail:] = torch.randn(tail, cols, device="cuda", generator=g).bfloat16()
+    assert rows * cols > 2 ** 31
+    nc, ns = fx.fp4_bytes(rows, cols, fmt)
+    codes, scales = torch.empty(nc, dtype=torch.uint8, device="cuda"), torch.empty(ns, dtype=torch.uint8, device="cuda")
+    q = fx.Fp4(codes.data_ptr(), scales.data_ptr(), rows, cols, fmt, 1.0)
+    small = Matrix(fx, tail, cols, fmt)
+    out, alone = torch.zeros_like(x), torch.zeros(tail, cols, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp4_quantize(x.data_ptr(), fx.BF16, cols, q)
+    ctx.fp4_dequantize(q, out.data_ptr(), fx.BF16, cols)
+    ctx.fp4_quantize(x[-tail:].data_ptr(), fx.BF16, cols, small.h)
+    ctx.fp4_dequantize(small.h, alone.data_ptr(), fx.BF16, cols)
+    ctx.sync()
+    ones = ref.values(*ref.quantize(np.ones((1, fmt)), fmt), fmt)[0, 0]  # 6 * e4m3(1 / 6) for blocks of 16
+    assert torch.equal(out[-tail:], alone) and (out[:-tail] == ones).all()
+    # as weights: the last columns of a product, its rows past 2^32 bytes with them
+    first = torch.randn(3, cols, device="cuda", generator=g).bfloat16()
+    a = Matrix(fx, 3, cols, fmt)
+    full, part = torch.zeros(3, rows, device="cuda"), torch.zeros(3, tail, device="cuda")
+    few, few_part = torch.zeros(3, rows, device="cuda"), torch.zeros(3, tail, device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp4_quantize(first.data_ptr(), fx.BF16, cols, a.h)
+    ctx.gemm_fp4(a.h, q, full.data_ptr(), fx.F32, rows)
+    ctx.gemm_fp4(a.h, small.h, part.data_ptr(), fx.F32, tail)
+    ctx.gemv_fp4(first.data_ptr(), fx.BF16, cols, 3, q, few.data_ptr(), fx.F32, rows)
+    ctx.gemv_fp4(first.data_ptr(), fx.BF16, cols, 3, small.h, few_part.data_ptr(), fx.F32, tail)
+    ctx.sync()
+    del x
+    # other splits of K: sums in another order, of 8192 products
+    scale = (first.float().abs().sum(1, keepdim=True) * 8.0)
+    assert ((full[:, -tail:] - part).abs() <= scale * 2.0 ** -18).all()
+    assert ((few[:, -tail:] - few_part).abs() <= scale * 2.0 ** -18).all()
+    # as rows, into an output of more than 2^31 elements
+    xa = Matrix(fx, rows, K, fmt)
+    rnd = torch.randn(rows, K, device="cuda", generator=g).bfloat16()
+    wa = Matrix(fx, cols, K, fmt)
+    wr = torch.randn(cols, K, device="cuda", generator=g).bfloat16()
+    torch.cuda.synchronize()
+    ctx.fp4_quantize(rnd.data_ptr(), fx.BF16, K, xa.h)
+    ctx.fp4_quantize(wr.data_ptr(), fx.BF16, K, wa.h)
+    ctx.gemm_fp4(xa.h, wa.h, out.data_ptr(), fx.BF16, cols)
+    last = Matrix(fx, tail, K, fmt)
+    ctx.fp4_quantize(rnd[-tail:].data_ptr(), fx.BF16, K, last.h)
+    ctx.gemm_fp4(last.h, wa.h, alone.data_ptr(), fx.BF16, cols)
+    ctx.sync()
+    assert torch.equal(out[-tail:], alone)  # one k-slice: the same sums
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_calls_run_on_the_contexts_device(fx):
+    """Whatever device is current, a context's calls run on its own, and leave the current one as it was."""
+    other = fx.Context(1)
+    torch.cuda.set_device(0)
+    x = torch.ones(4, 64, device="cuda:1")
+    codes, scales = torch.zeros(4 * 32, dtype=torch.uint8, device="cuda:1"), torch.zeros(512, dtype=torch.uint8, device="cuda:1")
+    q = fx.Fp4(codes.data_ptr(), scales.data_ptr(), 4, 64, 16, 1.0)
+    out = torch.zeros(4, 4, device="cuda:1")
+    torch.cuda.synchronize(1)
+    other.fp4_quantize(x.data_ptr(), fx.F32, 64, q)
+    other.gemm_fp4(q, q, out.data_ptr(), fx.F32, 4)
+    other.sync()
+    assert (out == 64).all() and torch.cuda.current_device() == 0
+    other.close()
+
+
 def test_two_contexts_at_once(fx, ctx):
     """Products on two contexts' streams at the same time share nothing."""
     other = fx.Context(0)
