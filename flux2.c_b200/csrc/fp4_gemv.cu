@@ -8,8 +8,9 @@
 // 2^(e + 126)) make two weights. Multiplying in f32 instead takes two conversions and one multiply-add per weight and row of x: measured 17 us
 // for one row and 36 for four (19456 x 2560), bound by instructions.
 //
-// Products: mma.sync m16n8k16 on bf16, 16 weight rows by up to 8 rows of x, f32 sums; x is split exactly into bf16 parts
-// (bf16 1, f16 2, f32 3), so every product is exact and up to 8 rows of x share one decoding. (tcgen05 wants its operands in
+// Products: mma.sync m16n8k16 on bf16, 16 weight rows by 8 columns, f32 sums. x is split exactly into bf16 parts (bf16 1,
+// f16 2, f32 3), each a column of its own, so every product is exact and all rows of x share one decoding (up to 32 columns,
+// more rows are further blocks). (tcgen05 wants its operands in
 // shared memory; decoded weights go from registers to the multiplication here.)
 //
 // A warp takes 32 weight rows at a time (a "unit": rows r + 32 q, r = 8 neighbours, q = 0..3, because one 16-byte piece of
@@ -28,6 +29,7 @@ namespace fx {
 
 static constexpr int V_WARPS = 16, V_THREADS = 32 * V_WARPS;  // one block per SM
 static constexpr int V_STEP_BYTES = 2 * 5 * 512;               // a warp's codes and factors of a step
+static_assert(V_STEP_BYTES >= 32 * 32 * 4, "32 columns of sums fit the places of a step");
 static constexpr int V_RING = 2 * V_WARPS * V_STEP_BYTES;      // two steps per warp
 static constexpr int V_SMEM_MAX = 227 * 1024 - V_RING;         // what is left for x and the sums
 
@@ -35,7 +37,7 @@ struct GemvFp4Params {
   const void *x;
   int x_vec;  // x and its row pitch are multiples of 16 bytes
   long long ldx;
-  int rows, group;  // rows of x; rows of x per block
+  int rows, group;  // rows of x; rows of x per block, each in PARTS columns
   const uint8_t *codes, *scales;
   long long pitch, chunks;
   float scale;
@@ -167,21 +169,21 @@ __device__ __forceinline__ void v_load8(const void *x, long long i, float (&v)[8
   }
 }
 
-// NH: 8 NH rows of x per block at most (group of them); PARTS: bf16 parts of x.
+// NH: 8 NH columns per block at most (group * PARTS of them, part by part); PARTS: bf16 parts of x.
 template <int NH, int PARTS, int BLOCK>
 __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_constant__ GemvFp4Params P) {
-  // the ring, then x [2 part_steps][PARTS][4][group][4], then sums [units + 2 V_WARPS][group][32]
+  // the ring, then x [2 part_steps][4][columns][4], then sums [units + 2 V_WARPS][group][32]
   extern __shared__ uint4 shared[];
   uint4 *xs = shared + V_RING / 16;
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int part = blockIdx.x % P.kparts, cluster = blockIdx.x / P.kparts;
-  const int G = P.group, m0 = blockIdx.y * G;
+  const int G = P.group, m0 = blockIdx.y * G, C = G * PARTS;
   const int s0 = static_cast<int>(static_cast<long long>(P.steps) * part / P.kparts),
             s1 = static_cast<int>(static_cast<long long>(P.steps) * (part + 1) / P.kparts), L = s1 - s0;
   const long long u0 = P.units * cluster / P.clusters;
   const int nu = static_cast<int>(P.units * (cluster + 1) / P.clusters - u0);
-  float *sums = reinterpret_cast<float *>(xs + 2 * P.part_steps * PARTS * 16 * G);
+  float *sums = reinterpret_cast<float *>(xs + 2 * P.part_steps * 16 * C);
 
   // this warp's stretch of the nu * L pairs, unit by unit
   auto begin_of = [&](int w) { return static_cast<int>(static_cast<long long>(nu) * L * w / V_WARPS); };
@@ -189,10 +191,10 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
   int u = first / L, st = first - u * L;
   VRows rows = v_rows<BLOCK>(P, u0 + (u < nu ? u : 0), s0 + st, lane);
   const int code_end = static_cast<int>(P.pitch), factor_end = static_cast<int>(P.chunks);
-  // lanes beyond the rows of x repeat the last one: the sums they take part in are dropped
+  // lanes beyond the columns repeat the last one: the sums they take part in are dropped
   int x_lane[NH];
 #pragma unroll
-  for (int nh = 0; nh < NH; ++nh) x_lane[nh] = (g + 8 * nh < G ? g + 8 * nh : G - 1) * 4 + t;
+  for (int nh = 0; nh < NH; ++nh) x_lane[nh] = (g + 8 * nh < C ? g + 8 * nh : C - 1) * 4 + t;
   const uint32_t ring = smem_u32(shared) + warp * 2 * V_STEP_BYTES + lane * 16;
   if (first < last) v_fetch<BLOCK>(ring, rows, s0 + st, t, code_end, factor_end);  // the weights do not wait for x
   for (int i = threadIdx.x; i < 2 * L * 16 * G; i += V_THREADS) {  // eight consecutive columns of a row
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
     for (int e = 0; e < 8; ++e) v_split<PARTS>(v[e], p[e]);
 #pragma unroll
     for (int h = 0; h < PARTS; ++h)  // columns i and i + 4 in a register, as the codes are decoded
-      xs[(((sx * PARTS + h) * 4 + jj) * G + m) * 4 + tt] = make_uint4(p[0][h] | p[4][h] << 16, p[1][h] | p[5][h] << 16,
+      xs[((sx * 4 + jj) * C + h * G + m) * 4 + tt] = make_uint4(p[0][h] | p[4][h] << 16, p[1][h] | p[5][h] << 16,
                                                                       p[2][h] | p[6][h] << 16, p[3][h] | p[7][h] << 16);
   }
   __syncthreads();
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
       const uint32_t fw[4] = {f4.x, f4.y, f4.z, f4.w};
       uint32_t m[4][2];
       uint32_t over[4];
-      bool wide = false;
+      bool wide = false;  // blocks of 32: a factor above 2, or NaN, somewhere in the warp
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (BLOCK == 16) {
@@ -257,14 +259,22 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
           m[q][1] = __byte_perm(__float_as_uint(f.y * 0x1p110f), 0, 0x3232);
         } else {
           const uint32_t b = fw[q] >> t * 8 & 0xFFu;
-          const uint32_t one = b == 255u ? 0x7FC0u : (min(b, 128u) + 126u) << 7;  // 2^(min(e, 1) + 126)
-          m[q][0] = m[q][1] = one * 0x10001u;
-          over[q] = ((b > 128u && b < 255u ? b - 1u : 127u) << 7) * 0x10001u;  // the rest of a factor above 2: 2^(e - 1)
+          m[q][0] = m[q][1] = (b + 126u) * 0x00800080u;  // 2^(e + 126), twice
           wide |= b > 128u;
         }
       }
-      if (BLOCK == 32) wide = __any_sync(0xffffffffu, wide);
-      const uint4 *xp = xs + (2 * st + half) * PARTS * 16 * G;
+      if (BLOCK == 32) {
+        wide = __any_sync(0xffffffffu, wide);
+        if (wide) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t b = fw[q] >> t * 8 & 0xFFu;
+            m[q][0] = m[q][1] = b == 255u ? 0x7FC07FC0u : (min(b, 128u) + 126u) * 0x00800080u;  // 2^(min(e, 1) + 126)
+            over[q] = (b > 128u && b < 255u ? b - 1u : 127u) * 0x00800080u;                     // the rest: 2^(e - 1)
+          }
+        }
+      }
+      const uint4 *xp = xs + (2 * st + half) * 16 * C;
       // The instruction truncates its sums: chains of more than 128 columns are added with rounding. (One chain over all of
       // K was 2.8e-6 off, relative, at K = 9216.)
       float e[2][NH][4];
@@ -281,13 +291,11 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
           }
         }
 #pragma unroll
-        for (int h = 0; h < PARTS; ++h)
-#pragma unroll
           for (int nh = 0; nh < NH; ++nh) {
-            const uint4 b = xp[(h * 4 + jj) * G * 4 + x_lane[nh]];
+            const uint4 b = xp[jj * C * 4 + x_lane[nh]];
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
-              if (jj + h == 0) v_mma0(e[tile][nh], a[2 * tile][0], a[2 * tile + 1][0], a[2 * tile][1], a[2 * tile + 1][1], b.x, b.y);
+              if (jj == 0) v_mma0(e[tile][nh], a[2 * tile][0], a[2 * tile + 1][0], a[2 * tile][1], a[2 * tile + 1][1], b.x, b.y);
               else v_mma(e[tile][nh], a[2 * tile][0], a[2 * tile + 1][0], a[2 * tile][1], a[2 * tile + 1][1], b.x, b.y);
               v_mma(e[tile][nh], a[2 * tile][2], a[2 * tile + 1][2], a[2 * tile][3], a[2 * tile + 1][3], b.z, b.w);
             }
@@ -302,15 +310,26 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
       }
     }
     st = 0;
+    // through the places of the step that was just used: the columns of a row of x are added, the smallest parts first
+    float *swap = reinterpret_cast<float *>(shared) + (warp * 2 + ((at - 1 - first) & 1)) * (V_STEP_BYTES / 4);
+    __syncwarp();
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
       for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int m = nh * 8 + 2 * t + (i & 1), q = 2 * tile + (i >> 1);
-          if (m < G) mine[m * 32 + q * 8 + g] = d[tile][nh][i];
+          const int c = nh * 8 + 2 * t + (i & 1), q = 2 * tile + (i >> 1);
+          if (c < C) swap[c * 32 + q * 8 + g] = d[tile][nh][i];
         }
+    __syncwarp();
+    for (int m = 0; m < G; ++m) {
+      float y = swap[((PARTS - 1) * G + m) * 32 + lane];
+#pragma unroll
+      for (int h = PARTS - 2; h >= 0; --h) y += swap[(h * G + m) * 32 + lane];
+      mine[m * 32 + lane] = y;
+    }
+    __syncwarp();
   }
   __syncthreads();
   // units in pieces: the pieces in the order of the warps (unit i is pairs [i L, i L + L))
@@ -372,7 +391,8 @@ static bool v_opt_in() {
 }
 int fp4_gemv_init(int device) {
   if (device < 0 || device >= 64) return -1;
-  if (!v_opt_in<1, 1>() || !v_opt_in<1, 2>() || !v_opt_in<1, 3>() || !v_opt_in<2, 1>() || !v_opt_in<2, 2>() || !v_opt_in<2, 3>())
+  if (!v_opt_in<1, 1>() || !v_opt_in<2, 1>() || !v_opt_in<1, 2>() || !v_opt_in<2, 2>() || !v_opt_in<4, 2>() || !v_opt_in<1, 3>() ||
+      !v_opt_in<2, 3>() || !v_opt_in<3, 3>() || !v_opt_in<4, 3>())
     return -2;
   for (int i = 0; i < 4; ++i) {
     cudaLaunchConfig_t cfg = {};
@@ -411,14 +431,15 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
   P.by = make_uint2((1u << 12) + (1u << 6), (1u << 8) + (1u << 2));
   P.units = fp4_row_tiles(w.rows) * 4;
   const int parts = x_dtype == FLUX_CUDA_BF16 ? 1 : x_dtype == FLUX_CUDA_F16 ? 2 : 3;
-  // Rows of x per block, and K in as many CTAs as it takes to fit them.
+  // Rows of x per block (evenly shared out, up to 32 columns), and K in as many CTAs as it takes to fit them.
+  const int blocks_of_rows = (rows * parts + 31) / 32;
+  P.group = (rows + blocks_of_rows - 1) / blocks_of_rows;
   auto x_bytes = [&](int group, int kparts) {
     return static_cast<long long>((P.steps + kparts - 1) / kparts) * 512 * parts * group;
   };
   const long long sums_room = 16384;
   P.kparts = 1;
-  while (P.kparts < 8 && P.kparts * 2 <= P.steps && x_bytes(rows, P.kparts) > V_SMEM_MAX - sums_room * (1 + (rows > 4))) P.kparts *= 2;
-  P.group = rows;
+  while (P.kparts < 8 && P.kparts * 2 <= P.steps && x_bytes(P.group, P.kparts) > V_SMEM_MAX - sums_room * (1 + (P.group > 4))) P.kparts *= 2;
   while (P.group > 1 && x_bytes(P.group, P.kparts) + (2 * V_WARPS + 1) * 128LL * P.group > V_SMEM_MAX) P.group = (P.group + 1) / 2;
   const int groups = (rows + P.group - 1) / P.group;
   // Of the ways to split K further, as long as a warp gets a step, the one that ends first: clusters at once, and how evenly
@@ -446,14 +467,19 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
   const dim3 grid(static_cast<unsigned>(clusters * P.kparts), groups);
   cudaError_t e;
 #define FX_V(NH, PARTS) e = w.format == 16 ? v_launch<NH, PARTS, 16>(grid, smem, st, P) : v_launch<NH, PARTS, 32>(grid, smem, st, P)
-  if (P.group <= 8) {
-    if (parts == 1) FX_V(1, 1);
-    else if (parts == 2) FX_V(1, 2);
-    else FX_V(1, 3);
+  const int nh = (P.group * parts + 7) / 8;
+  if (parts == 1) {
+    if (nh == 1) FX_V(1, 1);
+    else FX_V(2, 1);
+  } else if (parts == 2) {
+    if (nh == 1) FX_V(1, 2);
+    else if (nh == 2) FX_V(2, 2);
+    else FX_V(4, 2);
   } else {
-    if (parts == 1) FX_V(2, 1);
-    else if (parts == 2) FX_V(2, 2);
-    else FX_V(2, 3);
+    if (nh == 1) FX_V(1, 3);
+    else if (nh == 2) FX_V(2, 3);
+    else if (nh == 3) FX_V(3, 3);
+    else FX_V(4, 3);
   }
 #undef FX_V
   return e == cudaSuccess ? 0 : -8;
