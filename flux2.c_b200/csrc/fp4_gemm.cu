@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_con
     const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
     float mx = 0.f;
     const long long pitch = P.pitch, res_pitch = P.res_pitch;
-    uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * FP4_SIZE<DT>;
+    uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * static_cast<long long>(FP4_SIZE<DT>);
     const uint8_t *res = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + n * 4LL : nullptr;
     constexpr int STEP = 16;
     const bool direct = P.splits == 1 && n < P.N;
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_con
       if (ok) {
         const int first = live * rank / P.splits + q, end = live * (rank + 1) / P.splits, nj = n0 + lane * 4;
         const uint32_t mine = smem_u32(part) + lane * 16;
-        uint8_t *o = static_cast<uint8_t *>(P.out) + m0 * pitch + nj * FP4_SIZE<DT>;
+        uint8_t *o = static_cast<uint8_t *>(P.out) + m0 * pitch + nj * static_cast<long long>(FP4_SIZE<DT>);
         const uint8_t *r = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + nj * 4LL : nullptr;
         if (P.splits <= 2) fp4_join<DT, 2, 8>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
         else if (P.splits <= 4) fp4_join<DT, 4, 4>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
@@ -385,8 +385,12 @@ __global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_con
 
 // ------------------------------------------------------------------------------------------------
 // Large products: a pair of CTAs on neighbouring SMs owns a 256 (n) x 256 (m) tile. Each CTA stages its own 128 rows of w
-// and half (128) of the rows of x, so a k-slice costs an SM 38 KB of L2 traffic for 512 tensor cycles, which the L2 can
-// just deliver (a 128 x 256 tile per CTA would need 54 KB). The factors of x are needed in full by both CTAs.
+// and half (128) of the rows of x: 38 KB per k-slice and SM for 512 tensor cycles (a 128 x 256 tile per CTA would need 54
+// KB). The factors of x are needed in full by both CTAs. Bound by the delivery of operands: shared memory takes 600 cycles of
+// the slice (38 KB written, 32 KB read by the multiplications, 6 KB of factors copied, 128 bytes per cycle), and the L2
+// delivers 12 TB/s; a slice takes 822 cycles at 1500 MHz and 925 at 1965, so part of it does not follow the SM clock. At
+// 8192 x 8192 x 8192 (211 us) a sixth slice under way takes 224, without the factor copies it is 209, without the factors'
+// loads 206.
 //
 // TMEM holds 512 columns: two accumulators of 256 and 48 columns of factors do not fit, so the second accumulator starts
 // at column 208 and shares 48 columns with the first. The epilogue takes those columns first and releases the accumulator
@@ -522,7 +526,7 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
       const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
       const uint32_t acc = tmem + (t & 1) * C::ACC1 + (static_cast<uint32_t>(q * 32) << 16);
       const long long pitch = P.pitch, res_pitch = P.res_pitch;
-      uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * FP4_SIZE<DT>;
+      uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * static_cast<long long>(FP4_SIZE<DT>);
       const uint8_t *res = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + n * 4LL : nullptr;
       // Two warps share a lane group and take every other sixteen columns, in an order that starts with the columns the
       // accumulators share (the last 48 of the lower one, the first 48 of the upper one): once the first two loads of
