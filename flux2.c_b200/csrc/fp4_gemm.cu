@@ -207,13 +207,15 @@ __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m
 // One CTA per 128 (n) x BM (m) tile, or a cluster of `splits` CTAs that each take a part of K and add their parts in
 // rank order through distributed shared memory (no workspace, no atomics, the same bits every time).
 // ------------------------------------------------------------------------------------------------
-template <int BM, int BLOCK>
+// DEEP (the lowest tiles only): nine k-slices under way and one CTA per SM instead of four and two, for products whose few
+// CTAs each have that many slices: 1 x 2560 x 9728 then waits for memory once instead of twice.
+template <int BM, int BLOCK, bool DEEP>
 struct FCfg {
   static constexpr int CHUNKS = 256 / (4 * BLOCK);  // factor tiles per k-slice
   static constexpr int X_BYTES = BM * F_KB;
   static constexpr int S_BYTES = CHUNKS * 512;
   static constexpr int STAGE_BYTES = F_W_BYTES + X_BYTES + 2 * S_BYTES;
-  static constexpr int STAGES = BM >= 128 ? 3 : 4;
+  static constexpr int STAGES = DEEP ? 9 : BM >= 128 ? 3 : 4;
   static constexpr int SMEM = STAGES * STAGE_BYTES + 256;
   static constexpr int SF_COLS = CHUNKS * 4;
   static constexpr int TMEM_COLS = BM + 2 * SF_COLS <= 64 ? 64 : BM + 2 * SF_COLS <= 128 ? 128 : 256;
@@ -222,9 +224,9 @@ struct FCfg {
   static_assert(BM + 2 * SF_COLS <= TMEM_COLS, "accumulator and factors fit the allocation");
 };
 
-template <int BM, int BLOCK, int DT>
-__global__ void __launch_bounds__(F_THREADS, 2) gemm_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
-  using C = FCfg<BM, BLOCK>;
+template <int BM, int BLOCK, int DT, bool DEEP>
+__global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
+  using C = FCfg<BM, BLOCK, DEEP>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE_BYTES);
   uint64_t *empty = full + C::STAGES;
@@ -589,17 +591,16 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
 // ---------------------------------------------------------------------------------------------- host
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode4 = nullptr;
 
-template <int BM, int BLOCK>
-static cudaError_t opt_in() {
-  cudaError_t e = cudaFuncSetAttribute(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F32>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, FCfg<BM, BLOCK>::SMEM);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             FCfg<BM, BLOCK>::SMEM);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             FCfg<BM, BLOCK>::SMEM);
-  return e;
+template <int BM, int BLOCK, int DT, bool DEEP>
+static bool opt_in_one() {
+  return cudaFuncSetAttribute(gemm_fp4_kernel<BM, BLOCK, DT, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              FCfg<BM, BLOCK, DEEP>::SMEM) == cudaSuccess;
+}
+template <int BM, bool DEEP>
+static bool opt_in() {
+  return opt_in_one<BM, 16, FLUX_CUDA_F32, DEEP>() && opt_in_one<BM, 16, FLUX_CUDA_F16, DEEP>() &&
+         opt_in_one<BM, 16, FLUX_CUDA_BF16, DEEP>() && opt_in_one<BM, 32, FLUX_CUDA_F32, DEEP>() &&
+         opt_in_one<BM, 32, FLUX_CUDA_F16, DEEP>() && opt_in_one<BM, 32, FLUX_CUDA_BF16, DEEP>();
 }
 
 template <int BLOCK>
@@ -615,9 +616,28 @@ static cudaError_t opt_in_pair() {
   return e;
 }
 
-// Clusters of 1 to 8 CTAs of the 128-row kernel (two per SM, as the smaller ones) that a device holds at once: the GPCs'
-// numbers of SMs are no multiples of most sizes, so they are fewer than the SMs make.
+// Clusters of 1 to 8 CTAs that a device holds at once with one CTA per SM: the GPCs' numbers of SMs are no multiples of most
+// sizes, so they are fewer than the SMs make (33 of four, 15 of eight). The query counts one CTA per SM for the kernels of
+// which two fit as well; those are taken to fit twice.
 static int g_fp4_clusters[64][9];
+
+static void count_clusters(int *counts) {
+  for (int s = 1; s <= 8; ++s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024 / s * s);
+    cfg.blockDim = dim3(F_THREADS);
+    cfg.dynamicSmemBytes = FCfg<32, 16, true>::SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = s;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;  // none: this size is not used
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_fp4_kernel<32, 16, FLUX_CUDA_BF16, true>, &cfg) != cudaSuccess) cudaGetLastError();
+    counts[s] = s == 1 && n < 1 ? 1 : n;
+  }
+}
 
 int fp4_gemm_init(int device) {
   if (device < 0 || device >= 64) return -1;
@@ -628,26 +648,10 @@ int fp4_gemm_init(int device) {
     if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || !fn) return -1;
     g_encode4 = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   }
-  const bool ok = opt_in<16, 16>() == cudaSuccess && opt_in<16, 32>() == cudaSuccess && opt_in<32, 16>() == cudaSuccess &&
-                  opt_in<32, 32>() == cudaSuccess && opt_in<64, 16>() == cudaSuccess && opt_in<64, 32>() == cudaSuccess &&
-                  opt_in<128, 16>() == cudaSuccess && opt_in<128, 32>() == cudaSuccess &&
-                  opt_in_pair<16>() == cudaSuccess && opt_in_pair<32>() == cudaSuccess;
+  const bool ok = opt_in<16, false>() && opt_in<16, true>() && opt_in<32, false>() && opt_in<32, true>() && opt_in<64, false>() &&
+                  opt_in<128, false>() && opt_in_pair<16>() == cudaSuccess && opt_in_pair<32>() == cudaSuccess;
   if (!ok) return -2;
-  for (int s = 1; s <= 8; ++s) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1024 / s * s);
-    cfg.blockDim = dim3(F_THREADS);
-    cfg.dynamicSmemBytes = FCfg<128, 16>::SMEM;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = s;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;  // none: this size is not used
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_fp4_kernel<128, 16, FLUX_CUDA_BF16>, &cfg) != cudaSuccess) cudaGetLastError();
-    g_fp4_clusters[device][s] = s == 1 && n < 1 ? 1 : n;
-  }
+  count_clusters(g_fp4_clusters[device]);
   return 0;
 }
 
@@ -674,14 +678,15 @@ static int map_factors(CUtensorMap *m, const flux_cuda_fp4 &q, uint32_t chunks, 
   return r == CUDA_SUCCESS ? 0 : -4;
 }
 
-template <int BM, int BLOCK>
+template <int BM, int BLOCK, bool DEEP>
 static cudaError_t launch_one(const Fp4GemmParams &P, unsigned grid, int dtype, cudaStream_t st) {
-  const size_t smem = FCfg<BM, BLOCK>::SMEM;
+  const size_t smem = FCfg<BM, BLOCK, DEEP>::SMEM;
+  const dim3 g(grid), t(F_THREADS);
   if (dtype == FLUX_CUDA_F32)
-    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F32>, dim3(grid), dim3(F_THREADS), smem, st, P.splits, P);
+    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F32, DEEP>, g, t, smem, st, P.splits, P);
   if (dtype == FLUX_CUDA_F16)
-    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F16>, dim3(grid), dim3(F_THREADS), smem, st, P.splits, P);
-  return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_BF16>, dim3(grid), dim3(F_THREADS), smem, st, P.splits, P);
+    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F16, DEEP>, g, t, smem, st, P.splits, P);
+  return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_BF16, DEEP>, g, t, smem, st, P.splits, P);
 }
 
 template <int BLOCK>
@@ -697,38 +702,41 @@ static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype,
 // Which kernel, tile height and split a product gets: the least of the times below, in microseconds, whose constants are
 // measured on a B200 (148 SMs) and matter only relative to one another.
 //   One CTA per tile: 2.5 to start and stop, a k-slice 0.33 while the ring's latency bounds it (0.45 with the three stages
-//   of the 128-row tile) and its bytes over 12 TB/s of L2 when many CTAs run (a pitch off the 128-byte lines costs 1.6
-//   times as much), as many clusters at once as the device holds; a split adds a cluster launch and the exchange of the partial tile.
+//   of the 128-row tile; nine deep, 1.2 once and 0.06 per slice while they fit) and its bytes over 12 TB/s of L2 when many
+//   CTAs run (a pitch off the 128-byte lines costs 1.6 times as much), as many clusters at once as the device holds; a split
+//   adds a cluster launch and the exchange of the partial tile.
 //   Pairs: a k-slice 0.35, an epilogue of 2 that the next tile's products hide.
 // Measured at 1024 x 1024 x 1024: 64 rows 4.8, 128 rows 5.8, pairs 7.0; 512 x 2560 x 9728: 128 rows 20.8 alone, 16.2 split
-// three ways, pairs 19.2; 1 x 2560 x 9728: 16.0 alone, 6.1 split eight ways; 128 x 2560 x 2560: 64 rows 6.8 alone, 7.6 split
-// in two.
+// three ways, pairs 19.2; 1 x 2560 x 9728: 16.0 alone, 6.1 split six ways, 5.9 deep; 32 x 2560 x 9728: 7.7 split eight ways,
+// 6.9 six ways deep; 1 x 19456 x 2560: 8.1, deep 12.7; 128 x 2560 x 2560: 64 rows 6.8 alone, 7.6 split in two.
 struct Fp4Choice {
   int bm, splits;  // bm 256: pairs
+  bool deep;
 };
 static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_sms, const int *clusters) {
   const long long tn = (N + F_BN - 1) / F_BN;
-  Fp4Choice best = {128, 1};
+  Fp4Choice best = {128, 1, false};
   double least = 1e30;
   for (int bm = 16; bm <= 128; bm *= 2) {
     if (bm < 64 && M > bm) continue;  // a tile starts on half a factor tile at the least
     const long long tiles = tn * ((M + bm - 1) / bm);
-    for (int s = 1; s <= 8 && s <= slices; ++s) {
-      const long long at_once = clusters[s];
-      if (at_once < 1) continue;
-      const double active = static_cast<double>(tiles < at_once ? tiles : at_once) * s, waves = (tiles + at_once - 1) / at_once;
-      const double latency = bm == 128 ? 0.45 : 0.33;
-      const double bytes = active * (F_W_BYTES + bm * F_KB + 4096) / 12e6 * (pitch % 128 ? 1.6 : 1.0);
-      const double t = 2.5 + waves * ((slices + s - 1) / s) * (latency > bytes ? latency : bytes) +
-                       (s == 1 ? waves * bm * 0.012 : waves * (1.2 + 0.04 * bm));
-      if (t < least) least = t, best = {bm, s};
-    }
+    for (int deep = 0; deep <= (bm < 64); ++deep)
+      for (int s = 1; s <= 8 && s <= slices; ++s) {
+        const long long at_once = clusters[s] * (deep ? 1LL : 2LL);
+        if (at_once < 1) continue;
+        const int n = (slices + s - 1) / s;
+        const double active = static_cast<double>(tiles < at_once ? tiles : at_once) * s, waves = (tiles + at_once - 1) / at_once;
+        const double latency = deep ? 1.2 + (n <= 9 ? 0.06 : 0.15) * n : (bm == 128 ? 0.45 : 0.33) * n;
+        const double bytes = n * active * (F_W_BYTES + bm * F_KB + 4096) / 12e6 * (pitch % 128 ? 1.6 : 1.0);
+        const double t = 2.5 + waves * (latency > bytes ? latency : bytes) + (s == 1 ? waves * bm * 0.012 : waves * (1.0 + 0.05 * s + 0.04 * bm));
+        if (t < least) least = t, best = {bm, s, deep != 0};
+      }
     if (bm >= M) break;  // a taller tile would only be emptier
   }
   if (M > 128) {
     const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256), pairs = num_sms / 2;
     const double waves = (tiles + pairs - 1) / pairs, main = slices * 0.35 * (pitch % 128 ? 1.3 : 1.0) + 0.4;
-    if (2.5 + waves * (main > 2.0 ? main : 2.0) + 2.0 < least) best = {256, 1};
+    if (2.5 + waves * (main > 2.0 ? main : 2.0) + 2.0 < least) best = {256, 1, false};
   }
   return best;
 }
@@ -766,11 +774,13 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
   }
   const unsigned grid = static_cast<unsigned>(static_cast<long long>(P.tiles_m) * ((N + F_BN - 1) / F_BN) * P.splits);
   cudaError_t e;
-#define FX_G(BM) e = block == 16 ? launch_one<BM, 16>(P, grid, a.dtype, st) : launch_one<BM, 32>(P, grid, a.dtype, st)
-  if (bm == 16) FX_G(16);
-  else if (bm == 32) FX_G(32);
-  else if (bm == 64) FX_G(64);
-  else FX_G(128);
+#define FX_G(BM, DEEP) e = block == 16 ? launch_one<BM, 16, DEEP>(P, grid, a.dtype, st) : launch_one<BM, 32, DEEP>(P, grid, a.dtype, st)
+  if (bm == 16 && choice.deep) FX_G(16, true);
+  else if (bm == 16) FX_G(16, false);
+  else if (bm == 32 && choice.deep) FX_G(32, true);
+  else if (bm == 32) FX_G(32, false);
+  else if (bm == 64) FX_G(64, false);
+  else FX_G(128, false);
 #undef FX_G
   return e == cudaSuccess ? 0 : -8;
 }

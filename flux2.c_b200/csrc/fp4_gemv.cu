@@ -239,57 +239,57 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
       }
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
-      const uint32_t mine_at = ring + ((at - first) & 1) * V_STEP_BYTES + half * 5 * 512;
-      uint4 cur[4];
+        const uint32_t mine_at = ring + ((at - first) & 1) * V_STEP_BYTES + half * 5 * 512;
+        uint4 cur[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) cur[q] = v_ring(mine_at + q * 512);
-      const uint4 f4 = v_ring(mine_at + 4 * 512);
-      // this lane's factors: two blocks of 16 per row (half of a factor word), or one of 32 (a quarter of it)
-      const uint32_t fw[4] = {f4.x, f4.y, f4.z, f4.w};
-      uint32_t m[4][2];
-      uint32_t over[4];
-      bool wide = false;  // blocks of 32: a factor above 2, or NaN, somewhere in the warp
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (BLOCK == 16) {
-          uint32_t h;
-          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(fw[q] >> (t & 1) * 16)));
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-          m[q][0] = __byte_perm(__float_as_uint(f.x * 0x1p110f), 0, 0x3232);
-          m[q][1] = __byte_perm(__float_as_uint(f.y * 0x1p110f), 0, 0x3232);
-        } else {
-          const uint32_t b = fw[q] >> t * 8 & 0xFFu;
-          m[q][0] = m[q][1] = (b + 126u) * 0x00800080u;  // 2^(e + 126), twice
-          wide |= b > 128u;
-        }
-      }
-      if (BLOCK == 32) {
-        wide = __any_sync(0xffffffffu, wide);
-        if (wide) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t b = fw[q] >> t * 8 & 0xFFu;
-            m[q][0] = m[q][1] = b == 255u ? 0x7FC07FC0u : (min(b, 128u) + 126u) * 0x00800080u;  // 2^(min(e, 1) + 126)
-            over[q] = (b > 128u && b < 255u ? b - 1u : 127u) * 0x00800080u;                     // the rest: 2^(e - 1)
-          }
-        }
-      }
-      const uint4 *xp = xs + (2 * st + half) * 16 * C;
-      // The instruction truncates its sums: chains of more than 128 columns are added with rounding. (One chain over all of
-      // K was 2.8e-6 off, relative, at K = 9216.)
-      float e[2][NH][4];
-#pragma unroll
-      for (int jj = 0; jj < 4; ++jj) {
-        uint32_t a[4][4];
+        for (int q = 0; q < 4; ++q) cur[q] = v_ring(mine_at + q * 512);
+        const uint4 f4 = v_ring(mine_at + 4 * 512);
+        // this lane's factors: two blocks of 16 per row (half of a factor word), or one of 32 (a quarter of it)
+        const uint32_t fw[4] = {f4.x, f4.y, f4.z, f4.w};
+        uint32_t m[4][2];
+        uint32_t over[4];
+        bool wide = false;  // blocks of 32: a factor above 2, or NaN, somewhere in the warp
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t w = jj == 0 ? cur[q].x : jj == 1 ? cur[q].y : jj == 2 ? cur[q].z : cur[q].w;
-          v_decode(w, m[q][jj >> 1], P.by, a[q]);
-          if (BLOCK == 32 && wide) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[q][i] = v_mul2(a[q][i], over[q]);
+          if (BLOCK == 16) {
+            uint32_t h;
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(fw[q] >> (t & 1) * 16)));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+            m[q][0] = __byte_perm(__float_as_uint(f.x * 0x1p110f), 0, 0x3232);
+            m[q][1] = __byte_perm(__float_as_uint(f.y * 0x1p110f), 0, 0x3232);
+          } else {
+            const uint32_t b = fw[q] >> t * 8 & 0xFFu;
+            m[q][0] = m[q][1] = (b + 126u) * 0x00800080u;  // 2^(e + 126), twice
+            wide |= b > 128u;
           }
         }
+        if (BLOCK == 32) {
+          wide = __any_sync(0xffffffffu, wide);
+          if (wide) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t b = fw[q] >> t * 8 & 0xFFu;
+              m[q][0] = m[q][1] = b == 255u ? 0x7FC07FC0u : (min(b, 128u) + 126u) * 0x00800080u;  // 2^(min(e, 1) + 126)
+              over[q] = (b > 128u && b < 255u ? b - 1u : 127u) * 0x00800080u;                     // the rest: 2^(e - 1)
+            }
+          }
+        }
+        const uint4 *xp = xs + (2 * st + half) * 16 * C;
+        // The instruction truncates its sums: chains of more than 128 columns are added with rounding. (One chain over all of
+        // K was 2.8e-6 off, relative, at K = 9216.)
+        float e[2][NH][4];
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          uint32_t a[4][4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t w = jj == 0 ? cur[q].x : jj == 1 ? cur[q].y : jj == 2 ? cur[q].z : cur[q].w;
+            v_decode(w, m[q][jj >> 1], P.by, a[q]);
+            if (BLOCK == 32 && wide) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) a[q][i] = v_mul2(a[q][i], over[q]);
+            }
+          }
 #pragma unroll
           for (int nh = 0; nh < NH; ++nh) {
             const uint4 b = xp[jj * C * 4 + x_lane[nh]];
@@ -300,13 +300,13 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
               v_mma(e[tile][nh], a[2 * tile][2], a[2 * tile + 1][2], a[2 * tile][3], a[2 * tile + 1][3], b.z, b.w);
             }
           }
-      }
+        }
 #pragma unroll
-      for (int tile = 0; tile < 2; ++tile)
+        for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
-        for (int nh = 0; nh < NH; ++nh)
+          for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d[tile][nh][i] += e[tile][nh][i];
+            for (int i = 0; i < 4; ++i) d[tile][nh][i] += e[tile][nh][i];
       }
     }
     st = 0;
