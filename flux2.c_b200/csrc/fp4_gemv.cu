@@ -16,19 +16,19 @@
 // A warp takes 32 weight rows at a time (a "unit": rows r + 32 q, r = 8 neighbours, q = 0..3, because one 16-byte piece of
 // a factor tile holds the factors of exactly the rows r + 32 q for four blocks) in steps of 256 columns, a 128-byte line of
 // each row: a lane loads twice 32 consecutive codes of its four rows, and because sums do not care for order, those are its
-// columns in the multiplication too. The loads go to a ring in shared memory, asynchronously and each lane to places of its
-// own, so that a step is on its way while one is computed without costing registers or barriers; 64 bytes of a row at a
-// time into registers came to 2.1 TB/s. x lies in shared memory in the order of the multiplication's registers. K is split among the CTAs of a cluster, so that
-// x fits and the units of a cluster are many enough to be shared out evenly; the warps of a CTA take equal stretches
-// of its (unit, step) pairs, wherever these begin and end. Partial sums are added in a fixed order through (distributed)
-// shared memory: no workspace, no atomics, the same bits every time.
+// columns in the multiplication too. The loads go to a ring in shared memory, asynchronously and without barriers, so that a
+// step is on its way while one is computed without costing registers; 64 bytes of a row at a time into registers came to 2.1
+// TB/s. x lies in shared memory in the order of the multiplication's registers. K is split among the CTAs of a cluster, so
+// that x fits and the units of a cluster are many enough to be shared out evenly; the warps of a CTA take equal stretches of
+// its (unit, step) pairs, wherever these begin and end. Partial sums are added in a fixed order through (distributed) shared
+// memory: no workspace, no atomics, the same bits every time.
 #include "fp4.cuh"
 #include "launch.cuh"
 
 namespace fx {
 
 static constexpr int V_WARPS = 16, V_THREADS = 32 * V_WARPS;  // one block per SM
-static constexpr int V_STEP_BYTES = 2 * 5 * 512;               // a warp's codes and factors of a step
+static constexpr int V_STEP_BYTES = 8 * 512 + 512;             // a warp's codes and factors of a step
 static_assert(V_STEP_BYTES >= 32 * 32 * 4, "32 columns of sums fit the places of a step");
 static constexpr int V_RING = 2 * V_WARPS * V_STEP_BYTES;      // two steps per warp
 static constexpr int V_SMEM_MAX = 227 * 1024 - V_RING;         // what is left for x and the sums
@@ -73,20 +73,24 @@ __device__ __forceinline__ void v_copy16(uint32_t dst, const uint8_t *src, bool 
   if (in) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
 }
-// A step of a unit into this lane's places, [half of the step][4 rows of codes, factors][lane], and on to the next step.
-// left: bytes of codes and chunks of factors from the step's first column to the end of the row.
+// A step of a unit: the codes into this lane's places, [half of the step][4 rows][lane], and the pieces of factors into the
+// warp's, [half][piece][8 neighbours], by the first of the lanes that share one; and on to the next step. left, chunks: bytes
+// of codes and chunks of factors from here to the end of the row.
 template <int BLOCK>
-__device__ __forceinline__ void v_fetch(uint32_t dst, VRows &r, int step, int t, int code_end, int factor_end) {
-  const int left = code_end - step * 128 - t * 16, chunks = factor_end - step * (64 / BLOCK) - t * 8 / BLOCK;
+__device__ __forceinline__ void v_fetch(uint32_t dst, VRows &r, int step, int lane, int code_end, int factor_end) {
+  constexpr int PIECES = 32 / BLOCK;  // of half a step: two chunks of 64 columns, or one of 128
+  const int g = lane >> 2, t = lane & 3, p = t * 8 / BLOCK;
+  const int left = code_end - step * 128 - t * 16, chunks = factor_end - step * 2 * PIECES - p;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {  // half a step is 32 / BLOCK chunks: two of 64 columns, or one of 128
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v_copy16(dst + (h * 5 + q) * 512, r.codes[q] + h * 64, left > h * 64);
-    v_copy16(dst + (h * 5 + 4) * 512, r.factors + h * (32 / BLOCK) * 512, chunks > h * (32 / BLOCK));
+    for (int q = 0; q < 4; ++q) v_copy16(dst + (h * 4 + q) * 512 + lane * 16, r.codes[q] + h * 64, left > h * 64);
+    if (t * 8 % BLOCK == 0)
+      v_copy16(dst + 8 * 512 + ((h * PIECES + p) * 8 + g) * 16, r.factors + h * PIECES * 512, chunks > h * PIECES);
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) r.codes[q] += 128;
-  r.factors += (64 / BLOCK) * 512;
+  r.factors += 2 * PIECES * 512;
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 __device__ __forceinline__ uint4 v_ring(uint32_t addr) {
@@ -195,8 +199,9 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
   int x_lane[NH];
 #pragma unroll
   for (int nh = 0; nh < NH; ++nh) x_lane[nh] = (g + 8 * nh < C ? g + 8 * nh : C - 1) * 4 + t;
-  const uint32_t ring = smem_u32(shared) + warp * 2 * V_STEP_BYTES + lane * 16;
-  if (first < last) v_fetch<BLOCK>(ring, rows, s0 + st, t, code_end, factor_end);  // the weights do not wait for x
+  const uint32_t ring = smem_u32(shared) + warp * 2 * V_STEP_BYTES;
+  const uint32_t my_factors = 8 * 512 + (t * 8 / BLOCK * 8 + g) * 16;
+  if (first < last) v_fetch<BLOCK>(ring, rows, s0 + st, lane, code_end, factor_end);  // the weights do not wait for x
   for (int i = threadIdx.x; i < 2 * L * 16 * G; i += V_THREADS) {  // eight consecutive columns of a row
     const int c8 = i % (2 * L * 16), m = i / (2 * L * 16);
     const int sx = c8 >> 4, tt = (c8 >> 2) & 3, jj = c8 & 3;
@@ -232,18 +237,19 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
     for (; st < stop; ++st, ++at) {
       if (at + 1 < last) {
         if (st + 1 == L) rows = v_rows<BLOCK>(P, u0 + u + 1, s0, lane);
-        v_fetch<BLOCK>(ring + ((at + 1 - first) & 1) * V_STEP_BYTES, rows, s0 + (st + 1 == L ? 0 : st + 1), t, code_end, factor_end);
+        v_fetch<BLOCK>(ring + ((at + 1 - first) & 1) * V_STEP_BYTES, rows, s0 + (st + 1 == L ? 0 : st + 1), lane, code_end, factor_end);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
       } else {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
       }
+      __syncwarp();  // the factors were copied by other lanes; nobody overwrites them before the multiplications below
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
-        const uint32_t mine_at = ring + ((at - first) & 1) * V_STEP_BYTES + half * 5 * 512;
+        const uint32_t here = ring + ((at - first) & 1) * V_STEP_BYTES;
         uint4 cur[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) cur[q] = v_ring(mine_at + q * 512);
-        const uint4 f4 = v_ring(mine_at + 4 * 512);
+        for (int q = 0; q < 4; ++q) cur[q] = v_ring(here + (half * 4 + q) * 512 + lane * 16);
+        const uint4 f4 = v_ring(here + my_factors + half * (32 / BLOCK) * 128);
         // this lane's factors: two blocks of 16 per row (half of a factor word), or one of 32 (a quarter of it)
         const uint32_t fw[4] = {f4.x, f4.y, f4.z, f4.w};
         uint32_t m[4][2];
@@ -448,9 +454,11 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
     const long long n = g_clusters[device][kparts == 1 ? 0 : kparts == 2 ? 1 : kparts == 4 ? 2 : 3] / groups;
     return n < 1 ? 1 : n > P.units ? P.units : n;
   };
-  auto longest = [&](int kparts) {  // steps that the busiest warp of a cluster does, and a little for every part
-    const long long n = held(kparts), rows_of_steps = (P.units + n - 1) / n * ((P.steps + kparts - 1) / kparts);
-    return static_cast<double>((rows_of_steps + V_WARPS - 1) / V_WARPS) + 0.5 * (kparts > 1);
+  // in steps of a warp: what the busiest cluster's warps do, a quarter for joining parts, and laying out x (a fifth of a
+  // step for every 16 bytes and thread)
+  auto longest = [&](int kparts) {
+    const long long n = held(kparts), pairs = (P.units + n - 1) / n * ((P.steps + kparts - 1) / kparts);
+    return static_cast<double>(pairs) / V_WARPS + 0.25 * (kparts > 1) + 0.2 * x_bytes(P.group, kparts) / (16 * V_THREADS);
   };
   int split = P.kparts;
   for (int k = P.kparts * 2, i = P.kparts == 1 ? 1 : P.kparts == 2 ? 2 : 3; k <= 8 && k <= P.steps; k *= 2, ++i)

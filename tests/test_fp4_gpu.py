@@ -266,6 +266,8 @@ def _product(fx, ctx, M, N, K, fmt, out, gated=False, pad=0, in_place=False, sca
     (1, 1, 1), (1, 128, 64), (1, 130, 256), (1, 300, 2560), (2, 127, 31), (7, 129, 1111), (16, 256, 512), (17, 64, 257),
     (33, 128, 300), (64, 384, 1024), (65, 100, 96), (77, 1001, 1111), (128, 128, 256), (129, 257, 640), (200, 640, 1000),
     (256, 256, 2048), (300, 513, 96),
+    # low tiles with four and with nine k-slices under way, alone and split
+    (12, 2000, 9000), (16, 20000, 600), (24, 500, 6000), (30, 2560, 3000), (20, 19000, 300),
     # enough tiles for pairs of CTAs: ragged in every direction, one and several tiles per pair, many k-slices
     (1290, 2300, 70), (700, 3300, 300), (1025, 2049, 1600), (2600, 5200, 64), (150, 9600, 513)])
 def test_product_sizes(fx, ctx, M, N, K, fmt):
@@ -274,7 +276,8 @@ def test_product_sizes(fx, ctx, M, N, K, fmt):
 
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("gated,in_place", [(False, False), (True, False), (True, True)])
-@pytest.mark.parametrize("M,N,K,pad", [(3, 200, 500, 0), (100, 131, 260, 5), (140, 256, 3000, 8), (520, 700, 300, 1), (1300, 2200, 300, 4),
+@pytest.mark.parametrize("M,N,K,pad", [(3, 200, 500, 0), (100, 131, 260, 5), (140, 256, 3000, 8), (520, 700, 300, 1), (24, 260, 6000, 2), (16, 2560, 2560, 0),
+                                       (90, 128, 7000, 3), (1300, 2200, 300, 4),
                                        (1500, 6000, 296, 3)])
 def test_product_outputs(fx, ctx, M, N, K, pad, gated, in_place, out):
     if in_place and out != "f32":
