@@ -90,14 +90,12 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   return r;
 }
 
-// Codes of 16 columns and the factor byte of their block. For blocks of 32 the two threads of a block exchange their
-// maxima, so the whole warp must call this.
+// Codes of 16 columns and the factor byte of their block. inv_scale is a power of two, and the division by the matrix's scale
+// is exact whatever f32 makes of it: whether a block is finite is asked of x itself, and a quotient that f32 cannot hold is
+// either kept at the largest f32 (beyond it) or never formed (below it). For blocks of 32 the two threads of a block exchange
+// their maxima, so the whole warp must call this.
 template <int BLOCK>
 __device__ __forceinline__ uint32_t q_encode(float (&v)[16], float inv_scale, uint2 &codes) {
-  if (inv_scale != 1.0f) {
-#pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] *= inv_scale;
-  }
   float a = fabsf(v[0]);
 #pragma unroll
   for (int k = 1; k < 15; k += 2) a = max3_abs(a, v[k], v[k + 1]);
@@ -111,16 +109,38 @@ __device__ __forceinline__ uint32_t q_encode(float (&v)[16], float inv_scale, ui
   uint32_t byte;
   float q[16];
   if (BLOCK == 32) {
-    const int e = static_cast<int>(top >> 23) - 2;
-    byte = bad ? 255u : static_cast<uint32_t>(e > 0 ? e : 0);
-    const float r = bad ? 0.f : __uint_as_float((254u - byte) << 23);  // 2^-(byte - 127): the quotient is exact
+    // the factor's and the scale's powers of two in one, 2^-shift, so that the quotient is exact. (The exponent of a subnormal
+    // maximum is that of its product with 2^24; where no scale raises it, the factor is the least one anyway.)
+    const int k = 127 - static_cast<int>(__float_as_uint(inv_scale) >> 23);  // the scale is 2^k
+    int e = static_cast<int>(top >> 23) - 2;
+    if (e < 0 && k < 0) e = static_cast<int>(__float_as_uint(__uint_as_float(top) * 0x1p24f) >> 23) - 26;
+    e = top == 0 ? 0 : min(max(e - k, 0), 254);
+    byte = bad ? 255u : static_cast<uint32_t>(e);
+    const int shift = 127 - e - k;  // -125 .. 151
+    float r = bad ? 0.f : __uint_as_float(static_cast<uint32_t>(min(shift, 127) + 127) << 23);
+    if (shift > 127) {  // only tiny x: nothing overflows on the way
+      const float rest = __uint_as_float(static_cast<uint32_t>(shift) << 23);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= rest;
+    }
     const uint64_t r2 = f2_pack(r, r);
 #pragma unroll
-    for (int k = 0; k < 16; k += 2) f2_unpack(f2_mul(f2_pack(v[k], v[k + 1]), r2), q[k], q[k + 1]);
+    for (int i = 0; i < 16; i += 2) f2_unpack(f2_mul(f2_pack(v[i], v[i + 1]), r2), q[i], q[i + 1]);
   } else {
+    a = __uint_as_float(bad ? 0u : top);
+    if (inv_scale != 1.0f) {
+      a *= inv_scale;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] *= inv_scale;
+      if (a > 3.402823466e38f) {  // the largest factor, and codes of 6 for what is beyond f32
+        a = 3.402823466e38f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = fminf(fmaxf(v[k], -a), a);
+      }
+      // A quotient below the normal range is not exact, but its block has the factor 0 or its code is 0.
+    }
     // a / 6 rounded to odd (truncated, with the lowest bit set where something was cut off): rounding that to e4m3 is
     // rounding the exact quotient
-    a = __uint_as_float(bad ? 0u : top);
     float t = a * (1.0f / 6.0f);  // within one unit of a / 6; the residual's sign tells on which side
     const float rest = __fmaf_rn(-t, 6.0f, a);
     uint32_t bits = __float_as_uint(t);
