@@ -13,6 +13,8 @@
 // the end is zero codes and zero factors, so no size needs to be a multiple of anything.
 #include <cuda.h>
 #include <cudaTypedefs.h>
+#include <float.h>
+#include <math.h>
 #include <string.h>
 
 #include "fp4.cuh"
@@ -32,7 +34,8 @@ struct alignas(64) Fp4GemmParams {
   int M, N, slices;          // k-slices of 256 codes
   int tiles_m, tiles;
   int splits;                // CTAs of a cluster that share one output tile, each with its part of the k-slices
-  float alpha;
+  float alpha;               // x.scale * w.scale
+  float pre, pre2;           // STEPS: the same as two factors (fp4_alpha), and alpha is 1
   void *out;
   const float *gate, *residual;
   uint32_t pitch, res_pitch;  // bytes from row to row of out and residual
@@ -124,19 +127,28 @@ __device__ __forceinline__ void fp4_residual(float (&v)[16], int rows, const uin
       v[j] = j < rows ? __ldcg(reinterpret_cast<const float *>(res + static_cast<uint64_t>(res_pitch) * j)) : 0.f;
   }
 }
+// What a sum is multiplied by. STEPS = false: a = alpha * gate in one step, for calls without a gate or with alpha = 1, and
+// alpha a normal f32. Otherwise alpha * gate (or the scales' product) may leave the f32 range although the result does not, so
+// the sum is taken to x.scale * w.scale first and to a = gate then; a gate of 0 leaves nothing of a sum of any size.
+// Instances of their own, because the multiplications cost every other call 0.2 - 0.3 us of exposed epilogue, even behind a
+// branch (1024 x 6144 x 2560: 13.6 -> 13.9 us).
+template <bool STEPS>
+__device__ __forceinline__ float fp4_scaled(float sum, float a, float pre, float pre2) {
+  return STEPS ? sum * (a == 0.f ? 0.f : pre) * pre2 : sum;
+}
 // Epilogue of 16 output rows of this thread's column n, starting at `out`: a = alpha * gate, v the residual if any. Each row's
 // address is one multiply-add of its own (row pitches are 32 bits, checked on the host), and whole blocks carry no
 // predicates: one warp per scheduler has nothing to hide a chain of 64-bit additions or a branch behind. Checked and
 // addressed row by row a store cost 150 cycles, along a chain 32.
-template <int DT>
+template <int DT, bool STEPS>
 __device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], float (&v)[16], bool residual, int rows, uint8_t *out,
-                                         uint32_t pitch, float a, float &mx) {
+                                         uint32_t pitch, float a, float pre, float pre2, float &mx) {
   if (residual) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = fmaf(a, __uint_as_float(r[j]), v[j]);
+    for (int j = 0; j < 16; ++j) v[j] = fmaf(a, fp4_scaled<STEPS>(__uint_as_float(r[j]), a, pre, pre2), v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = a * __uint_as_float(r[j]);
+    for (int j = 0; j < 16; ++j) v[j] = a * fp4_scaled<STEPS>(__uint_as_float(r[j]), a, pre, pre2);
   }
   if (rows >= 16) {
     if (DT == FLUX_CUDA_F32) {
@@ -160,10 +172,10 @@ __device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], float (&v)[16]
 // The second half of a split tile: rows [m, m_end) of the tile, every fourth one this warp's, four neighbouring columns
 // per lane, the parts of up to SP CTAs added in rank order. R rows' parts (16 loads) are requested before the first is
 // used: a load from another SM takes most of a microsecond.
-template <int DT, int SP, int R>
+template <int DT, int SP, int R, bool STEPS>
 __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m_end, int n, int N, uint8_t *out,
-                                         long long pitch, const uint8_t *res, long long res_pitch, float alpha,
-                                         const float *gate, float &mx) {
+                                         long long pitch, const uint8_t *res, long long res_pitch, float alpha, float pre,
+                                         float pre2, const float *gate, float &mx) {
   float g[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) g[i] = gate && n + i < N ? alpha * gate[n + i] : alpha;
@@ -190,10 +202,10 @@ __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m
 #pragma unroll
       for (int s = 1; s < SP; ++s)
         if (s < splits) a.x += v[s][j].x, a.y += v[s][j].y, a.z += v[s][j].z, a.w += v[s][j].w;
-      y[j][0] = fmaf(g[0], a.x, y[j][0]);
-      y[j][1] = fmaf(g[1], a.y, y[j][1]);
-      y[j][2] = fmaf(g[2], a.z, y[j][2]);
-      y[j][3] = fmaf(g[3], a.w, y[j][3]);
+      y[j][0] = fmaf(g[0], fp4_scaled<STEPS>(a.x, g[0], pre, pre2), y[j][0]);
+      y[j][1] = fmaf(g[1], fp4_scaled<STEPS>(a.y, g[1], pre, pre2), y[j][1]);
+      y[j][2] = fmaf(g[2], fp4_scaled<STEPS>(a.z, g[2], pre, pre2), y[j][2]);
+      y[j][3] = fmaf(g[3], fp4_scaled<STEPS>(a.w, g[3], pre, pre2), y[j][3]);
     }
 #pragma unroll
     for (int j = 0; j < R; ++j)
@@ -224,7 +236,7 @@ struct FCfg {
   static_assert(BM + 2 * SF_COLS <= TMEM_COLS, "accumulator and factors fit the allocation");
 };
 
-template <int BM, int BLOCK, int DT, bool DEEP>
+template <int BM, int BLOCK, int DT, bool DEEP, bool STEPS>
 __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
   using C = FCfg<BM, BLOCK, DEEP>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -344,7 +356,7 @@ __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const
         } else if (direct) {
           float next[16];
           if (res) fp4_residual(next, live - c - STEP, res + (c + STEP) * res_pitch, P.res_pitch);
-          fp4_emit<DT>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, mx);
+          fp4_emit<DT, STEPS>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, P.pre, P.pre2, mx);
           if (res) {
 #pragma unroll
             for (int j = 0; j < STEP; ++j) v[j] = next[j];
@@ -361,9 +373,9 @@ __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const
         const uint32_t mine = smem_u32(part) + lane * 16;
         uint8_t *o = static_cast<uint8_t *>(P.out) + m0 * pitch + nj * static_cast<long long>(FP4_SIZE<DT>);
         const uint8_t *r = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + nj * 4LL : nullptr;
-        if (P.splits <= 2) fp4_join<DT, 2, 8>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
-        else if (P.splits <= 4) fp4_join<DT, 4, 4>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
-        else fp4_join<DT, 8, 2>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.gate, mx);
+        if (P.splits <= 2) fp4_join<DT, 2, 8, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.pre, P.pre2, P.gate, mx);
+        else if (P.splits <= 4) fp4_join<DT, 4, 4, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.pre, P.pre2, P.gate, mx);
+        else fp4_join<DT, 8, 2, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.pre, P.pre2, P.gate, mx);
       }
     }
     sat_report(P.err + 1, DT == FLUX_CUDA_F16, mx);
@@ -412,7 +424,7 @@ struct F2Cfg {
   static_assert(SFB + 8 * CHUNKS <= 512 && ACC1 + 256 <= SFA && ACC1 + SHARED == 256, "TMEM columns");
 };
 
-template <int BLOCK, int DT>
+template <int BLOCK, int DT, bool STEPS>
 __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_constant__ Fp4GemmParams P) {
   using C = F2Cfg<BLOCK>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -540,7 +552,7 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
       float v0[16], v1[16];
       auto column = [&](int i) { return (shared + 16 * (2 * i + half)) & 255; };
       auto finish = [&](const uint32_t (&r)[16], float (&v)[16], int c) {
-        fp4_emit<DT>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, mx);
+        fp4_emit<DT, STEPS>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, P.pre, P.pre2, mx);
       };
       auto fetch = [&](float (&v)[16], int c) {
         if (res) fp4_residual(v, live - c, res + c * res_pitch, P.res_pitch);
@@ -593,8 +605,11 @@ static PFN_cuTensorMapEncodeTiled_v12000 g_encode4 = nullptr;
 
 template <int BM, int BLOCK, int DT, bool DEEP>
 static bool opt_in_one() {
-  return cudaFuncSetAttribute(gemm_fp4_kernel<BM, BLOCK, DT, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              FCfg<BM, BLOCK, DEEP>::SMEM) == cudaSuccess;
+  const int smem = FCfg<BM, BLOCK, DEEP>::SMEM;
+  return cudaFuncSetAttribute(gemm_fp4_kernel<BM, BLOCK, DT, DEEP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+             cudaSuccess &&
+         cudaFuncSetAttribute(gemm_fp4_kernel<BM, BLOCK, DT, DEEP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+             cudaSuccess;
 }
 template <int BM, bool DEEP>
 static bool opt_in() {
@@ -603,17 +618,18 @@ static bool opt_in() {
          opt_in_one<BM, 32, FLUX_CUDA_F16, DEEP>() && opt_in_one<BM, 32, FLUX_CUDA_BF16, DEEP>();
 }
 
+template <int BLOCK, int DT>
+static bool opt_in_pair_one() {
+  const int smem = F2Cfg<BLOCK>::SMEM;
+  return cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, DT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+             cudaSuccess &&
+         cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, DT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+             cudaSuccess;
+}
 template <int BLOCK>
-static cudaError_t opt_in_pair() {
-  cudaError_t e = cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       F2Cfg<BLOCK>::SMEM);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             F2Cfg<BLOCK>::SMEM);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             F2Cfg<BLOCK>::SMEM);
-  return e;
+static bool opt_in_pair() {
+  return opt_in_pair_one<BLOCK, FLUX_CUDA_F32>() && opt_in_pair_one<BLOCK, FLUX_CUDA_F16>() &&
+         opt_in_pair_one<BLOCK, FLUX_CUDA_BF16>();
 }
 
 // Clusters of 1 to 8 CTAs that a device holds at once with one CTA per SM: the GPCs' numbers of SMs are no multiples of most
@@ -634,7 +650,7 @@ static void count_clusters(int *counts) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;  // none: this size is not used
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_fp4_kernel<32, 16, FLUX_CUDA_BF16, true>, &cfg) != cudaSuccess) cudaGetLastError();
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_fp4_kernel<32, 16, FLUX_CUDA_BF16, true, false>, &cfg) != cudaSuccess) cudaGetLastError();
     counts[s] = s == 1 && n < 1 ? 1 : n;
   }
 }
@@ -649,7 +665,7 @@ int fp4_gemm_init(int device) {
     g_encode4 = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   }
   const bool ok = opt_in<16, false>() && opt_in<16, true>() && opt_in<32, false>() && opt_in<32, true>() && opt_in<64, false>() &&
-                  opt_in<128, false>() && opt_in_pair<16>() == cudaSuccess && opt_in_pair<32>() == cudaSuccess;
+                  opt_in<128, false>() && opt_in_pair<16>() && opt_in_pair<32>();
   if (!ok) return -2;
   count_clusters(g_fp4_clusters[device]);
   return 0;
@@ -678,25 +694,32 @@ static int map_factors(CUtensorMap *m, const flux_cuda_fp4 &q, uint32_t chunks, 
   return r == CUDA_SUCCESS ? 0 : -4;
 }
 
-template <int BM, int BLOCK, bool DEEP>
-static cudaError_t launch_one(const Fp4GemmParams &P, unsigned grid, int dtype, cudaStream_t st) {
+template <int BM, int BLOCK, bool DEEP, bool STEPS>
+static cudaError_t launch_steps(const Fp4GemmParams &P, unsigned grid, int dtype, cudaStream_t st) {
   const size_t smem = FCfg<BM, BLOCK, DEEP>::SMEM;
   const dim3 g(grid), t(F_THREADS);
   if (dtype == FLUX_CUDA_F32)
-    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F32, DEEP>, g, t, smem, st, P.splits, P);
+    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F32, DEEP, STEPS>, g, t, smem, st, P.splits, P);
   if (dtype == FLUX_CUDA_F16)
-    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F16, DEEP>, g, t, smem, st, P.splits, P);
-  return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_BF16, DEEP>, g, t, smem, st, P.splits, P);
+    return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_F16, DEEP, STEPS>, g, t, smem, st, P.splits, P);
+  return launch_kernel(gemm_fp4_kernel<BM, BLOCK, FLUX_CUDA_BF16, DEEP, STEPS>, g, t, smem, st, P.splits, P);
+}
+template <int BM, int BLOCK, bool DEEP>
+static cudaError_t launch_one(const Fp4GemmParams &P, unsigned grid, int dtype, bool steps, cudaStream_t st) {
+  return steps ? launch_steps<BM, BLOCK, DEEP, true>(P, grid, dtype, st) : launch_steps<BM, BLOCK, DEEP, false>(P, grid, dtype, st);
 }
 
-template <int BLOCK>
-static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype, cudaStream_t st) {
+template <int BLOCK, bool STEPS>
+static cudaError_t launch_pair_steps(const Fp4GemmParams &P, unsigned grid, int dtype, cudaStream_t st) {
   const size_t smem = F2Cfg<BLOCK>::SMEM;
-  if (dtype == FLUX_CUDA_F32)
-    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F32>, dim3(grid), dim3(F2_THREADS), smem, st, 2, P);
-  if (dtype == FLUX_CUDA_F16)
-    return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F16>, dim3(grid), dim3(F2_THREADS), smem, st, 2, P);
-  return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16>, dim3(grid), dim3(F2_THREADS), smem, st, 2, P);
+  const dim3 g(grid), t(F2_THREADS);
+  if (dtype == FLUX_CUDA_F32) return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F32, STEPS>, g, t, smem, st, 2, P);
+  if (dtype == FLUX_CUDA_F16) return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_F16, STEPS>, g, t, smem, st, 2, P);
+  return launch_kernel(gemm2_fp4_kernel<BLOCK, FLUX_CUDA_BF16, STEPS>, g, t, smem, st, 2, P);
+}
+template <int BLOCK>
+static cudaError_t launch_pair(const Fp4GemmParams &P, unsigned grid, int dtype, bool steps, cudaStream_t st) {
+  return steps ? launch_pair_steps<BLOCK, true>(P, grid, dtype, st) : launch_pair_steps<BLOCK, false>(P, grid, dtype, st);
 }
 
 // Which kernel, tile height and split a product gets: the least of the times below, in microseconds, whose constants are
@@ -741,6 +764,21 @@ static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_s
   return best;
 }
 
+// The two scales as factors that a sum is multiplied by one after the other: their product and 1, or, where f32 has no normal
+// number for the product, two that take the sum the same way, so that it leaves the f32 range only if the result does.
+static void fp4_alpha(float x, float w, float &first, float &second) {
+  const double both = static_cast<double>(x) * w;  // exact
+  first = static_cast<float>(both), second = 1.0f;
+  if (both == 0 || (fabsf(first) >= FLT_MIN && fabsf(first) <= FLT_MAX)) return;
+  if ((fabsf(x) >= 1.0f) == (fabsf(w) >= 1.0f)) {
+    first = x, second = w;
+  } else {  // a subnormal scale against one that is at least 1
+    int e;
+    const double m = frexp(both, &e);
+    first = ldexpf(static_cast<float>(m), e / 2), second = ldexpf(1.0f, e - e / 2);
+  }
+}
+
 int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cudaStream_t st) {
   Fp4GemmParams P;
   memset(&P, 0, sizeof(P));
@@ -758,7 +796,9 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
   P.slices = slices;
   P.tiles_m = (M + bm - 1) / bm;
   P.splits = choice.splits;
-  P.alpha = a.x.scale * a.w.scale;
+  fp4_alpha(a.x.scale, a.w.scale, P.pre, P.pre2);
+  const bool steps = P.pre2 != 1.0f || (a.gate && P.pre != 1.0f);
+  P.alpha = steps ? 1.0f : P.pre;
   P.out = a.out;
   P.pitch = static_cast<uint32_t>(a.ld_out * (a.dtype == FLUX_CUDA_F32 ? 4 : 2));
   P.gate = a.gate;
@@ -769,12 +809,15 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
     const long long pair_tiles = static_cast<long long>(P.tiles_m) * ((N + 255) / 256);
     P.tiles = static_cast<int>(pair_tiles);
     const int pairs = pair_tiles < num_sms / 2 ? P.tiles : num_sms / 2;
-    cudaError_t e = block == 16 ? launch_pair<16>(P, 2 * pairs, a.dtype, st) : launch_pair<32>(P, 2 * pairs, a.dtype, st);
+    cudaError_t e = block == 16 ? launch_pair<16>(P, 2 * pairs, a.dtype, steps, st)
+                                 : launch_pair<32>(P, 2 * pairs, a.dtype, steps, st);
     return e == cudaSuccess ? 0 : -8;
   }
   const unsigned grid = static_cast<unsigned>(static_cast<long long>(P.tiles_m) * ((N + F_BN - 1) / F_BN) * P.splits);
   cudaError_t e;
-#define FX_G(BM, DEEP) e = block == 16 ? launch_one<BM, 16, DEEP>(P, grid, a.dtype, st) : launch_one<BM, 32, DEEP>(P, grid, a.dtype, st)
+#define FX_G(BM, DEEP)                                                      \
+  e = block == 16 ? launch_one<BM, 16, DEEP>(P, grid, a.dtype, steps, st) \
+                  : launch_one<BM, 32, DEEP>(P, grid, a.dtype, steps, st)
   if (bm == 16 && choice.deep) FX_G(16, true);
   else if (bm == 16) FX_G(16, false);
   else if (bm == 32 && choice.deep) FX_G(32, true);

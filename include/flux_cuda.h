@@ -493,7 +493,8 @@ int flux_cuda_fp4_dequantize(flux_cuda_ctx *ctx, const flux_cuda_fp4 *q, void *o
 /*
  * out[m, n] = residual[m, n] + gate[n] * sum_k x[m, k] w[n, k] on the block-scaled tensor-core path: the 4-bit form of
  * flux_cuda_gemm_bf16's STORE and GATED_RES epilogues. x [M, K], w [N, K] of one format; any M, N >= 0, K >= 1. out of
- * `dtype` with row pitch ld_out; f32 sums, rounded once (f16 saturates and is counted). gate f32 [N] or NULL (1);
+ * `dtype` with row pitch ld_out; f32 sums of code * factor, then the two scales (whose product may lie outside f32), rounded
+ * once (f16 saturates and is counted). gate f32 [N] or NULL (1);
  * residual f32 [M, N] with row pitch ld_residual, or NULL (0); it may be `out` itself in f32 with the same pitch,
  * otherwise no output may overlap an input. Row pitches are below 2^30 elements. A NaN factor makes the products of its row or column NaN.
  */

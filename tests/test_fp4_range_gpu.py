@@ -55,3 +55,86 @@ def test_quantize_with_every_size_of_scale(fx, ctx, k, name, fmt):
     assert clean
     assert (byte == wbyte).all()
     assert np.array_equal(ref.values(code, byte, fmt), ref.values(want, wbyte, fmt), equal_nan=True)
+
+
+# ---------------------------------------------------------------------------------------------------- products
+def _exact_matrix(fx, rng, rows, cols, fmt, e, scale):
+    """Codes of 0, +-0.5 .. +-6 under one power-of-two factor 2^e: any sum of a few thousand products of two of them is an
+    exact f32 number. The last row is 0. -> the matrix and its values without the scale."""
+    code = rng.integers(0, 16, (rows, cols))
+    code[-1] = 0
+    nb = -(-cols // fmt)
+    b = (e + 127) if fmt == 32 else (e + 7) << 3
+    byte = np.full((rows, nb), b, np.uint8)
+    return Matrix(fx, rows, cols, fmt, scale, ref.pack(code, byte)), ref.values(code, byte, fmt)
+
+
+def _f32(v):
+    """float64 -> the nearest f32, infinity beyond it."""
+    with np.errstate(over="ignore"):
+        return v.astype(np.float32).astype(np.float64)
+
+
+SHAPES = [(5, 130, 600), (1, 40, 64), (24, 260, 6000), (130, 300, 3000), (1300, 2200, 300)]  # alone, split, in pairs of CTAs
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("fmt,ex,ew,sx,sw", [
+    (16, 0, 0, 2.0 ** 70, 2.0 ** 70),               # beyond f32, but for the rows and columns of zeros
+    (16, -6, -6, 2.0 ** 60, 2.0 ** 70),             # only the scales' product is
+    (32, -60, -60, 2.0 ** 100, 2.0 ** 100),
+    (32, -60, -60, -2.0 ** 127, 2.0 ** 65),
+    (32, 40, 40, 2.0 ** -100, 2.0 ** -60),          # only the scales' product is below it
+    (32, 50, 50, 2.0 ** -100, 2.0 ** -100),
+    (32, 50, 50, 2.0 ** -149, 2.0 ** -40),
+    (32, 20, 20, 1.7 * 2.0 ** -140, 1.3 * 2.0 ** 5),  # neither is, but the product has few digits left
+    (32, 0, 20, 2.0 ** 100, 1.9 * 2.0 ** -149),
+    (16, 3, 3, 2.0 ** -100, 2.0 ** -100),           # nothing is left
+    (16, 2, -2, 0.75, 1.7), (32, 100, -100, 2.0 ** 30, 2.0 ** -31), (16, 0, 0, 0.0, 2.0 ** 100)])
+def test_product_with_every_size_of_scale(fx, ctx, fmt, ex, ew, sx, sw, M, N, K):
+    """The sum times the two scales, whatever f32 makes of the scales' own product. The sums are exact; then at most three
+    roundings of 2^-24, and half of the smallest step where the result is subnormal."""
+    rng = np.random.default_rng(M + N + K)
+    x, xv = _exact_matrix(fx, rng, M, K, fmt, ex, sx)
+    w, wv = _exact_matrix(fx, rng, N, K, fmt, ew, sw)
+    out = torch.full((M + 1, N), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemm_fp4(x.h, w.h, out.data_ptr(), fx.F32, N)
+    ctx.sync()
+    want = (xv @ wv.T) * (float(np.float32(sx)) * float(np.float32(sw)))
+    got = out[:M].double().cpu().numpy()
+    assert (out[M:] == 7).all()
+    beyond = np.isinf(_f32(want))
+    assert (got[beyond] == np.sign(want[beyond]) * np.inf).all()
+    fine = ~beyond
+    assert (np.abs(got - want)[fine] <= 3 * 2.0 ** -24 * np.abs(want)[fine] + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("fmt,ex,ew,sx,sw,eg", [
+    (32, 40, 40, 2.0 ** -50, 2.0 ** -50, -35),   # scales * gate has few digits left
+    (32, 40, 40, 2.0 ** -60, 2.0 ** -60, -100),  # or none
+    (32, -50, -50, 2.0 ** 50, 2.0 ** 50, 40),    # or is beyond f32
+    (32, -60, -60, 2.0 ** 100, 2.0 ** 100, -70),
+    (32, 50, 50, 2.0 ** -100, 2.0 ** -100, 70),
+    (16, 0, 0, 0.5, 1.7, 0)])
+def test_gated_product_with_every_size_of_scale(fx, ctx, fmt, ex, ew, sx, sw, eg, in_place, M, N, K):
+    """gate and residual: one rounding more, and that of the sum with the residual. A gate of 0 leaves the residual."""
+    rng = np.random.default_rng(M + N + K + 1)
+    x, xv = _exact_matrix(fx, rng, M, K, fmt, ex, sx)
+    w, wv = _exact_matrix(fx, rng, N, K, fmt, ew, sw)
+    gate = (rng.uniform(1, 2, N) * rng.choice([-1, 1], N) * 2.0 ** eg).astype(np.float32)
+    gate[::7] = 0
+    term = gate.astype(np.float64) * ((xv @ wv.T) * (float(np.float32(sx)) * float(np.float32(sw))))
+    residual = (rng.standard_normal((M, N)) * np.abs(term).mean()).astype(np.float32)
+    want = residual.astype(np.float64) + term
+    g, r = torch.from_numpy(gate).cuda(), torch.from_numpy(residual).cuda()
+    out = r.clone() if in_place else torch.zeros(M, N, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemm_fp4(x.h, w.h, out.data_ptr(), fx.F32, N, gate_ptr=g.data_ptr(),
+                 residual_ptr=out.data_ptr() if in_place else r.data_ptr(), ld_residual=N)
+    ctx.sync()
+    got = out.double().cpu().numpy()
+    assert (np.abs(got - want) <= 4 * 2.0 ** -24 * np.abs(term) + 2.0 ** -24 * np.abs(want) + 2.0 ** -149).all()
+    assert (got[:, ::7] == residual[:, ::7]).all()
