@@ -22,6 +22,8 @@
 // that x fits and the units of a cluster are many enough to be shared out evenly; the warps of a CTA take equal stretches of
 // its (unit, step) pairs, wherever these begin and end. Partial sums are added in a fixed order through (distributed) shared
 // memory: no workspace, no atomics, the same bits every time.
+#include <math.h>
+
 #include "fp4.cuh"
 #include "launch.cuh"
 
@@ -40,7 +42,7 @@ struct GemvFp4Params {
   int rows, group;  // rows of x; rows of x per block, each in PARTS columns
   const uint8_t *codes, *scales;
   long long pitch, chunks;
-  float scale;
+  float scale, scale2;  // what a sum is multiplied by; the second is 1 unless f32 cannot hold the two as one
   int N, K, steps;  // steps of 256 columns
   int kparts;       // K is split among this many CTAs of a cluster
   int part_steps;   // most steps of a CTA
@@ -373,8 +375,8 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
     }
     const long long unit_i = u0 + u, n = (unit_i >> 2) * 128 + (unit_i & 3) * 8 + (rl & 7) + 32 * (rl >> 3);
     if (n < P.N && m0 + m < P.rows) {
-      if (BLOCK == 16) y *= 65536.0f;  // the factors went in as factor * 2^110, against codes * 2^-126
       y *= P.scale;
+      if (P.scale2 != 1.0f) y *= P.scale2;
       const long long at = (m0 + m) * P.ld + n;
       if (P.dt == FLUX_CUDA_F32) fp4_store<FLUX_CUDA_F32>(P.out, at, y, mx);
       else if (P.dt == FLUX_CUDA_F16) fp4_store<FLUX_CUDA_F16>(P.out, at, y, mx);
@@ -431,7 +433,11 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
   P.x_vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !(ldx * (x_dtype == FLUX_CUDA_F32 ? 4 : 2) & 15);
   P.codes = static_cast<const uint8_t *>(w.codes), P.scales = static_cast<const uint8_t *>(w.scales);
   P.pitch = fp4_pitch(w.cols), P.chunks = fp4_chunks(w.cols, w.format);
-  P.scale = w.scale, P.N = w.rows, P.K = w.cols;
+  // Blocks of 16: the factors go in as factor * 2^110, against codes * 2^-126. In one step with the scale, because the sum
+  // times 2^16 may be beyond f32 where the result is not.
+  P.scale = w.format == 16 ? w.scale * 65536.0f : w.scale, P.scale2 = 1.0f;
+  if (isinf(P.scale)) P.scale = w.scale, P.scale2 = 65536.0f;
+  P.N = w.rows, P.K = w.cols;
   P.steps = (w.cols + 255) / 256;
   P.out = out, P.dt = dtype, P.ld = ld_out, P.sat = sat;
   P.by = make_uint2((1u << 12) + (1u << 6), (1u << 8) + (1u << 2));

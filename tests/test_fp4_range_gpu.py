@@ -138,3 +138,23 @@ def test_gated_product_with_every_size_of_scale(fx, ctx, fmt, ex, ew, sx, sw, eg
     got = out.double().cpu().numpy()
     assert (np.abs(got - want) <= 4 * 2.0 ** -24 * np.abs(term) + 2.0 ** -24 * np.abs(want) + 2.0 ** -149).all()
     assert (got[:, ::7] == residual[:, ::7]).all()
+
+
+# ---------------------------------------------------------------------------------------------------- few rows
+@pytest.mark.parametrize("xname", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt,e,ex,scale", [
+    (16, 7, 120, 2.0 ** -60), (16, 7, 120, 2.0 ** -100), (16, -6, -100, 2.0 ** 125), (16, 0, -100, 2.0 ** 127),
+    (32, 7, 100, 2.0 ** -60), (32, -20, -80, 2.0 ** 127), (32, 100, -90, 2.0 ** -100), (16, 0, 100, 2.0 ** -149)])
+def test_few_row_product_with_every_size_of_scale(fx, ctx, fmt, e, ex, scale, xname):
+    """The matrix's scale comes to the sum in one step: sums that it brings back into the f32 range are not lost before.
+    x of one code's step and codes under one factor: exact sums and, by a power of two, exact results."""
+    rng = np.random.default_rng(7)
+    w, wv = _exact_matrix(fx, rng, 70, 200, fmt, e, scale)
+    dev, x = _plain(rng.integers(-3, 4, (5, 200)) * 2.0 ** ex, xname, 200)
+    out = torch.zeros(5, 70, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemv_fp4(dev.data_ptr(), _dt(fx, xname), 200, 5, w.h, out.data_ptr(), fx.F32, 70)
+    ctx.sync()
+    want = (x @ wv.T) * scale
+    assert np.isfinite(_f32(want)).all()
+    assert (np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -149).all()
