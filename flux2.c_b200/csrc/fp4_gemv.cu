@@ -8,7 +8,7 @@
 // 2^(e + 126)) make two weights. Multiplying in f32 instead takes two conversions and one multiply-add per weight and row of x: measured 17 us
 // for one row and 36 for four (19456 x 2560), bound by instructions.
 //
-// Products: mma.sync m16n8k16 on bf16, 16 weight rows by 8 columns, f32 sums. x is split exactly into bf16 parts (bf16 1,
+// Products: mma.sync m16n8k16 on bf16, 16 weight rows by 8 columns, f32 sums. x is split into bf16 parts (bf16 1,
 // f16 2, f32 3), each a column of its own, so every product is exact and all rows of x share one decoding (up to 32 columns,
 // more rows are further blocks). (tcgen05 wants its operands in
 // shared memory; decoded weights go from registers to the multiplication here.)
@@ -134,7 +134,11 @@ __device__ __forceinline__ void v_mma0(float (&d)[4], uint32_t a0, uint32_t a1, 
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// The exact bf16 parts of a value, the largest first (8 bits of the magnitude each).
+// The bf16 parts of a value, the largest first (8 bits of the magnitude each), the second times 2^7 and the third times 2^15:
+// as they are the lower parts of numbers below 2^-110 would lie among the subnormal bf16 numbers, whose digits end at 2^-133.
+// Taken up so far a part is not above the value itself, so no sum leaves f32 earlier; of f32 numbers below 2^-124 the digit
+// 2^-149 is cut off.
+__device__ __forceinline__ constexpr float v_up(int part) { return part == 0 ? 128.f : 256.f; }  // from one part to the next
 template <int PARTS>
 __device__ __forceinline__ void v_split(float x, uint32_t (&p)[PARTS]) {
   const bool finite = (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
@@ -143,7 +147,7 @@ __device__ __forceinline__ void v_split(float x, uint32_t (&p)[PARTS]) {
   for (int i = 0; i < PARTS; ++i) {
     const uint32_t top = __float_as_uint(x) & 0xFFFF0000u;
     p[i] = top >> 16;
-    x = finite ? x - __uint_as_float(top) : 0.f;
+    x = finite ? (x - __uint_as_float(top)) * v_up(i) : 0.f;
   }
 }
 
@@ -334,7 +338,7 @@ __global__ void __launch_bounds__(V_THREADS, 1) gemv_fp4_kernel(const __grid_con
     for (int m = 0; m < G; ++m) {
       float y = swap[((PARTS - 1) * G + m) * 32 + lane];
 #pragma unroll
-      for (int h = PARTS - 2; h >= 0; --h) y += swap[(h * G + m) * 32 + lane];
+      for (int h = PARTS - 2; h >= 0; --h) y = fmaf(y, 1.0f / v_up(h), swap[(h * G + m) * 32 + lane]);
       mine[m * 32 + lane] = y;
     }
     __syncwarp();

@@ -502,7 +502,7 @@ int flux_cuda_gemm_fp4(flux_cuda_ctx *ctx, const flux_cuda_fp4 *x, const flux_cu
                        long long ld_out, const float *gate, const float *residual, long long ld_residual);
 /*
  * The same product for 0 .. 16 rows of x that stay as they are (x_dtype, row pitch ldx): out[m, n] = sum_k x[m, k]
- * w[n, k], f32 sums of exact products. For single tokens and modulation vectors, where reading the weights is the whole
+ * w[n, k], f32 sums of exact products (w without its scale; of NVFP4 held times 2^-16, so that they end at 2^-133). For single tokens and modulation vectors, where reading the weights is the whole
  * cost. Up to 65536 columns.
  */
 int flux_cuda_gemv_fp4(flux_cuda_ctx *ctx, const void *x, int x_dtype, long long ldx, int rows, const flux_cuda_fp4 *w,

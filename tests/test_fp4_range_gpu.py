@@ -158,3 +158,23 @@ def test_few_row_product_with_every_size_of_scale(fx, ctx, fmt, e, ex, scale, xn
     want = (x @ wv.T) * scale
     assert np.isfinite(_f32(want)).all()
     assert (np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("fmt,e", [(32, 100), (32, 125), (32, 0), (16, 7)])
+@pytest.mark.parametrize("ex", [-149, -140, -130, -126, -122, -118, -110, -100])
+def test_few_row_product_of_tiny_rows(fx, ctx, ex, fmt, e):
+    """f32 x down to the smallest subnormal numbers keeps its digits where the weights make something of it, but for the digit
+    2^-149. Sums as in test_fp4_gpu._few_row_tolerance for 64 columns, with steps of 2^-149 (blocks of 16, whose sums are held
+    times 2^-16: 2^-133) per product below the normal range."""
+    rng = np.random.default_rng(ex + 500)
+    K = 64
+    w, wv = _exact_matrix(fx, rng, 40, K, fmt, e, 1.0)
+    dev, x = _plain(rng.uniform(1, 2, (4, K)) * rng.choice([-1, 1], (4, K)) * 2.0 ** ex, "f32", K)
+    out = torch.zeros(4, 40, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemv_fp4(dev.data_ptr(), fx.F32, K, 4, w.h, out.data_ptr(), fx.F32, 40)
+    ctx.sync()
+    want = x @ wv.T
+    mag = np.abs(x) @ np.abs(wv).T
+    tol = mag * (2 * 3 * 4 + 8) * 2.0 ** -23 + 2.0 ** -149 * np.abs(wv).sum(1) + 3 * K * (2.0 ** -133 if fmt == 16 else 2.0 ** -149)
+    assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
