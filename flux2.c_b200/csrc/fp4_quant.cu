@@ -14,6 +14,8 @@
 // 128 to 256 bytes of loads in flight per thread, and of the factors exactly what lies in one 16-byte piece of a factor
 // tile, so the four lanes of a chunk put a piece together with shuffles and store it whole. No shared memory, no barrier:
 // rows beyond the last cost one predicate, which keeps a single token at the price of a launch.
+#include <math.h>
+
 #include "fp4.cuh"
 
 namespace fx {
@@ -267,18 +269,76 @@ int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda
 }
 
 // ------------------------------------------------------------------------------------------------
-// The values a 4-bit matrix stands for: the product with the matrix's own scale is rounded to f32 and then to the output
-// type, everything else is exact. Same tiling as above; bound by writing the values.
+// The values a 4-bit matrix stands for, rounded once. Same tiling as above; bound by writing the values.
+//
+// PLAIN scales are 0 and the normal powers of two: code * factor * scale in two multiplications is exact, or, for results
+// below f32's normal range, rounded once more only where a 16-bit type has 0 anyway. Under any other scale the product has
+// up to 30 bits, and rounding it to f32 on the way to a 16-bit type may put it on the middle between two values that it is
+// not on. It is rounded to odd then (truncated, with the lowest bit set where something was cut off), which later roundings to
+// fewer bits cannot tell from the exact product. The scale's power of two stays out of that and joins the factor's.
+// Measured at 9728 x 9216: to bf16 38.6 us (37.0 under a plain scale), blocks of 32 to f16 42.5 (36.8); f32 needs no second
+// rounding: 28.7 us at 4096 x 9216 (29.9).
 // ------------------------------------------------------------------------------------------------
-// Eight codes as f32 values times two factors, one after the other.
-__device__ __forceinline__ void dq_values(uint32_t c, float first, float second, float *v) {
+struct DqScale {
+  float scale, mant;  // scale = mant * 2^exp with 1 <= |mant| < 2
+  int exp;
+};
+// Two products a b rounded to odd; minus_b is -b.
+__device__ __forceinline__ void dq_odd(uint64_t a, uint64_t b, uint64_t minus_b, float &lo, float &hi) {
+  uint64_t p;
+  asm("mul.rz.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+  float cut_lo, cut_hi;
+  f2_unpack(p, lo, hi);
+  f2_unpack(f2_fma(a, minus_b, p), cut_lo, cut_hi);  // exact
+  if (cut_lo != 0.f) lo = __uint_as_float(__float_as_uint(lo) | 1u);
+  if (cut_hi != 0.f) hi = __uint_as_float(__float_as_uint(hi) | 1u);
+}
+// value * mant * 2^k where that may be no normal f32.
+template <int DT>
+__device__ __noinline__ float dq_far(float value, float mant, int k) {
+  const double d = static_cast<double>(value) * mant * __longlong_as_double(static_cast<long long>(k + 1023) << 52);  // exact
+  if (DT == FLUX_CUDA_F32) return __double2float_rn(d);
+  const float f = __double2float_rz(d);
+  return static_cast<double>(f) == d ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+// Eight codes under a factor's byte as f32 values that are to be rounded to the type.
+template <int DT, int BLOCK, bool PLAIN>
+__device__ __forceinline__ void dq_values(uint32_t c, uint32_t byte, const DqScale &S, float *v) {
   uint32_t h[4];
   fp4_unpack8(c, h);
+  const float s = fp4_factor<BLOCK>(byte);
+  if (PLAIN) {
+    // code * e4m3 is exact. A power of two may take a code out of the f32 range that a small scale brings back: then the
+    // scale comes first.
+    const bool scale_first = BLOCK == 32 && fabsf(S.scale) < 1.0f;
+    const float first = scale_first ? S.scale : s, second = scale_first ? s : S.scale;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
-    v[2 * j] = f.x * first * second;
-    v[2 * j + 1] = f.y * first * second;
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+      v[2 * j] = f.x * first * second;
+      v[2 * j + 1] = f.y * first * second;
+    }
+    return;
+  }
+  const float factor = BLOCK == 16 || byte == 255 ? s : 1.0f;
+  int k = BLOCK == 16 || byte == 255 ? S.exp : S.exp + static_cast<int>(byte) - 127;
+  if (!(c & 0x77777777u)) k = 0;  // zeros, those past the end of the matrix among them
+  if (k >= -100 && k <= 110) {    // mant * code (* e4m3) is within 2^-10 .. 2^13: normal products, and exact rests of them
+    const float two = factor * __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
+    const uint64_t two2 = f2_pack(two, two), mant2 = f2_pack(S.mant, S.mant), minus2 = f2_pack(-S.mant, -S.mant);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+      const uint64_t value = f2_mul(f2_pack(f.x, f.y), two2);
+      if (DT == FLUX_CUDA_F32) f2_unpack(f2_mul(value, mant2), v[2 * j], v[2 * j + 1]);
+      else dq_odd(value, mant2, minus2, v[2 * j], v[2 * j + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j / 2]));
+      v[j] = dq_far<DT>((j & 1 ? f.y : f.x) * factor, S.mant, k);
+    }
   }
 }
 
@@ -293,10 +353,10 @@ struct OutElement<FLUX_CUDA_F32> {
 
 // VEC: out and its row pitch are multiples of 32 bytes: 16 columns per thread in stores of 32 bytes. Otherwise the lanes of
 // a warp store neighbouring columns, so that the stores of an odd pitch still fill whole sectors.
-template <int DT, int BLOCK, bool VEC>
+template <int DT, int BLOCK, bool VEC, bool PLAIN>
 __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t *__restrict__ codes, long long pitch,
                                                                    const uint8_t *__restrict__ scales, long long chunks,
-                                                                   int rows, int cols, float scale, void *__restrict__ out,
+                                                                   int rows, int cols, DqScale S, void *__restrict__ out,
                                                                    long long ld, int col_tiles, int *sat) {
   pdl_launch_dependents();
   const int ct = blockIdx.x % col_tiles, rg = blockIdx.x / col_tiles % 4;
@@ -318,17 +378,13 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const long long r = r0 + 32 * q;
-    // code * e4m3 is exact. A power of two may take a code out of the f32 range that a small scale brings back: then the
-    // scale comes first.
-    const float s = fp4_factor<BLOCK>(fw[q] & 0xFFu);
-    const bool scale_first = BLOCK == 32 && fabsf(scale) < 1.0f;
-    const float first = scale_first ? scale : s, second = scale_first ? s : scale;
+    const uint32_t byte = fw[q] & 0xFFu;
     float top = 0.f;
     if (VEC && c0 + 16 <= cols) {
       if (r >= rows) continue;
       float v[16];
-      dq_values(cd[q].x, first, second, v);
-      dq_values(cd[q].y, first, second, v + 8);
+      dq_values<DT, BLOCK, PLAIN>(cd[q].x, byte, S, v);
+      dq_values<DT, BLOCK, PLAIN>(cd[q].y, byte, S, v + 8);
       char *p = reinterpret_cast<char *>(out) + (r * ld + c0) * FP4_SIZE<DT>;
       uint32_t w[Raw16<DT>::N];
 #pragma unroll
@@ -342,8 +398,8 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t
     } else if (VEC) {
       if (r >= rows || c0 >= cols) continue;
       float v[16];
-      dq_values(cd[q].x, first, second, v);
-      dq_values(cd[q].y, first, second, v + 8);
+      dq_values<DT, BLOCK, PLAIN>(cd[q].x, byte, S, v);
+      dq_values<DT, BLOCK, PLAIN>(cd[q].y, byte, S, v + 8);
 #pragma unroll
       for (int k = 0; k < 16; ++k)
         if (c0 + k < cols) fp4_store<DT>(out, r * ld + c0 + k, v[k], mx);
@@ -352,8 +408,8 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t
       using E = typename OutElement<DT>::T;
       __shared__ __align__(16) E stage[Q_THREADS / 32][2][Q_COLS];
       float v[16];
-      dq_values(cd[q].x, first, second, v);
-      dq_values(cd[q].y, first, second, v + 8);
+      dq_values<DT, BLOCK, PLAIN>(cd[q].x, byte, S, v);
+      dq_values<DT, BLOCK, PLAIN>(cd[q].y, byte, S, v + 8);
       const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
       uint4 *mine = reinterpret_cast<uint4 *>(&stage[warp][lane >> 4][cx * 16]);
       uint32_t w[Raw16<DT>::N];
@@ -385,23 +441,35 @@ int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long lon
   const bool vec = !(reinterpret_cast<uintptr_t>(out) & 31) && !((ld * size) & 31);
   const uint8_t *codes = static_cast<const uint8_t *>(q.codes), *scales = static_cast<const uint8_t *>(q.scales);
   const long long pitch = fp4_pitch(q.cols), chunks = fp4_chunks(q.cols, q.format);
-#define FX_D(DT, BL, AL)                                                                                                   \
-  fp4_dequantize_kernel<DT, BL, AL><<<static_cast<unsigned>(blocks), Q_THREADS, 0, st>>>(codes, pitch, scales, chunks, q.rows, \
-                                                                                         q.cols, q.scale, out, ld, col_tiles, sat)
-#define FX_D2(DT)                                  \
-  do {                                             \
-    if (q.format == 16) {                          \
-      if (vec) FX_D(DT, 16, true);                 \
-      else FX_D(DT, 16, false);                    \
-    } else {                                       \
-      if (vec) FX_D(DT, 32, true);                 \
-      else FX_D(DT, 32, false);                    \
-    }                                              \
+  DqScale S = {q.scale, 0.f, 0};
+  bool plain = true;
+  if (q.scale != 0.f) {
+    S.mant = 2.0f * frexpf(q.scale, &S.exp), --S.exp;
+    plain = fabsf(S.mant) == 1.0f && S.exp >= -126;
+  }
+#define FX_D(DT, BL, AL, PL)                                                                             \
+  fp4_dequantize_kernel<DT, BL, AL, PL><<<static_cast<unsigned>(blocks), Q_THREADS, 0, st>>>(           \
+      codes, pitch, scales, chunks, q.rows, q.cols, S, out, ld, col_tiles, sat)
+#define FX_D1(DT, BL, AL)            \
+  do {                               \
+    if (plain) FX_D(DT, BL, AL, true); \
+    else FX_D(DT, BL, AL, false);    \
+  } while (0)
+#define FX_D2(DT)                   \
+  do {                              \
+    if (q.format == 16) {           \
+      if (vec) FX_D1(DT, 16, true); \
+      else FX_D1(DT, 16, false);    \
+    } else {                        \
+      if (vec) FX_D1(DT, 32, true); \
+      else FX_D1(DT, 32, false);    \
+    }                               \
   } while (0)
   if (dtype == FLUX_CUDA_F32) FX_D2(FLUX_CUDA_F32);
   else if (dtype == FLUX_CUDA_F16) FX_D2(FLUX_CUDA_F16);
   else FX_D2(FLUX_CUDA_BF16);
 #undef FX_D2
+#undef FX_D1
 #undef FX_D
   return cudaGetLastError() == cudaSuccess ? 0 : -8;
 }

@@ -178,3 +178,67 @@ def test_few_row_product_of_tiny_rows(fx, ctx, ex, fmt, e):
     mag = np.abs(x) @ np.abs(wv).T
     tol = mag * (2 * 3 * 4 + 8) * 2.0 ** -23 + 2.0 ** -149 * np.abs(wv).sum(1) + 3 * K * (2.0 ** -133 if fmt == 16 else 2.0 ** -149)
     assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+
+
+# ---------------------------------------------------------------------------------------------------- reading back
+def _round_once(v, name):
+    """float64 -> the nearest value of a type, ties to even, as float64; f16 saturates."""
+    p, low, top = {"f32": (24, -126, F32_MAX), "f16": (11, -14, 65504.0),
+                   "bf16": (8, -126, float(torch.finfo(torch.bfloat16).max))}[name]
+    e = np.maximum(np.frexp(v)[1] - 1, low).astype(np.float64)
+    step = np.exp2(e - (p - 1))
+    r = np.round(v / step) * step
+    return np.where(np.abs(r) > top, np.sign(r) * (65504.0 if name == "f16" else np.inf), r)
+
+
+def _scales_next_to_ties():
+    """f32 scales whose product with 3 lies next to the middle of two neighbours of a 16-bit type, nearer than an f32 can
+    tell: 3 s = t +- 1/4 unit of f32, t such a middle."""
+    out = []
+    for bits in (8, 11):
+        cut = 24 - bits
+        for top in range(2 ** (bits - 1), 2 ** bits, 2 ** (bits - 1) // 64):
+            for odd, d in ((0, 1), (1, -1)):  # a tie would go to the even neighbour; this does not
+                t = (((top | 1) - 1 + odd) << cut | 1 << (cut - 1)) * 4 + d
+                if t % 3 == 0:
+                    out.append(t // 3 * 2.0 ** -24)
+    return [s for s in out if float(np.float32(s)) == s]
+
+
+def _read_back(fx, ctx, m, rows, cols, name, pad):
+    out = torch.zeros(rows, cols + pad, dtype=TORCH[name], device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp4_dequantize(m.h, out.data_ptr(), _dt(fx, name), cols + pad)
+    ctx.sync()
+    return out[:, :cols].double().cpu().numpy()
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -60, 2.0 ** 90, 0.3, -1.7, 1.1 * 2.0 ** -100, 1.9 * 2.0 ** -120, 1.3 * 2.0 ** 100,
+                                   F32_MAX, 2.0 ** -126, 3 * 2.0 ** -149, 2.0 ** -149, 1.234 * 2.0 ** -135, 0.0])
+def test_dequantize_rounds_once(fx, ctx, scale, name, fmt):
+    """Every code with every factor and a matrix scale from anywhere in the f32 range: the nearest value of the type, also
+    among the subnormal ones."""
+    code = np.tile(np.arange(16), (256, fmt // 16 * 3))
+    byte = np.repeat(np.arange(256)[:, None], 3, 1).astype(np.uint8)
+    if fmt == 16:
+        byte &= 127
+    m = Matrix(fx, 256, code.shape[1], fmt, scale, ref.pack(code, byte))
+    want = _round_once(ref.values(code, byte, fmt, float(np.float32(scale))), name)
+    for pad in (0, 1):
+        got = _read_back(fx, ctx, m, 256, code.shape[1], name, pad)
+        assert np.array_equal(got, want, equal_nan=True)
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_dequantize_next_to_ties(fx, ctx, name, fmt):
+    scales = _scales_next_to_ties()
+    assert len(scales) >= 40
+    code = np.tile(np.arange(16), (4, 4))
+    byte = np.tile(np.array([127, 128, 120, 126] if fmt == 32 else [0x38, 0x30, 0x3C, 0x48])[:, None], (1, 64 // fmt)).astype(np.uint8)
+    for s in scales:
+        m = Matrix(fx, 4, 64, fmt, s, ref.pack(code, byte))
+        want = _round_once(ref.values(code, byte, fmt, s), name)
+        assert (_read_back(fx, ctx, m, 4, 64, name, 0) == want).all()
