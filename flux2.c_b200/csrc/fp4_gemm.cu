@@ -736,7 +736,7 @@ struct Fp4Choice {
   int bm, splits;  // bm 256: pairs
   bool deep;
 };
-static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_sms, const int *clusters) {
+static Fp4Choice fp4_choose(long long M, long long N, int slices, long long pitch, int num_sms, const int *clusters) {
   const long long tn = (N + F_BN - 1) / F_BN;
   Fp4Choice best = {128, 1, false};
   double least = 1e30;
@@ -746,7 +746,7 @@ static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_s
     for (int deep = 0; deep <= (bm < 64); ++deep)
       for (int s = 1; s <= 8 && s <= slices; ++s) {
         const long long at_once = clusters[s] * (deep ? 1LL : 2LL);
-        if (at_once < 1) continue;
+        if (at_once < 1 || tiles * s > 0x7FFFFFFF) continue;  // the latter: more CTAs than a launch takes
         const int n = (slices + s - 1) / s;
         const double active = static_cast<double>(tiles < at_once ? tiles : at_once) * s, waves = (tiles + at_once - 1) / at_once;
         const double latency = deep ? 1.2 + (n <= 9 ? 0.06 : 0.15) * n : (bm == 128 ? 0.45 : 0.33) * n;
@@ -757,7 +757,7 @@ static Fp4Choice fp4_choose(int M, int N, int slices, long long pitch, int num_s
     if (bm >= M) break;  // a taller tile would only be emptier
   }
   if (M > 128) {
-    const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256), pairs = num_sms / 2;
+    const long long tiles = (M + 255) / 256 * ((N + 255) / 256), pairs = num_sms / 2;
     const double waves = (tiles + pairs - 1) / pairs, main = slices * 0.35 * (pitch % 128 ? 1.3 : 1.0) + 0.4;
     if (2.5 + waves * (main > 2.0 ? main : 2.0) + 2.0 < least) best = {256, 1, false};
   }
@@ -782,7 +782,8 @@ static void fp4_alpha(float x, float w, float &first, float &second) {
 int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cudaStream_t st) {
   Fp4GemmParams P;
   memset(&P, 0, sizeof(P));
-  const int M = a.x.rows, N = a.w.rows, block = a.x.format;
+  const long long M = a.x.rows, N = a.w.rows;  // up to 2^31 - 1: rounding up to tiles wants more bits
+  const int block = a.x.format;
   const int slices = static_cast<int>((static_cast<long long>(a.x.cols) + 255) / 256);
   const Fp4Choice choice = fp4_choose(M, N, slices, fp4_pitch(a.x.cols), num_sms, g_fp4_clusters[device]);
   const int bm = choice.bm;
@@ -791,10 +792,10 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
   if (map_codes(&P.tm_w, a.w, F_BN) || map_codes(&P.tm_x, a.x, pair ? 128 : bm) || map_factors(&P.tm_ws, a.w, chunks, 1) ||
       map_factors(&P.tm_xs, a.x, chunks, pair ? 2 : 1))
     return -4;
-  P.M = M;
-  P.N = N;
+  P.M = a.x.rows;
+  P.N = a.w.rows;
   P.slices = slices;
-  P.tiles_m = (M + bm - 1) / bm;
+  P.tiles_m = static_cast<int>((M + bm - 1) / bm);
   P.splits = choice.splits;
   fp4_alpha(a.x.scale, a.w.scale, P.pre, P.pre2);
   const bool steps = P.pre2 != 1.0f || (a.gate && P.pre != 1.0f);
@@ -806,14 +807,14 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
   P.res_pitch = static_cast<uint32_t>(a.ld_residual * 4);
   P.err = err;
   if (pair) {
-    const long long pair_tiles = static_cast<long long>(P.tiles_m) * ((N + 255) / 256);
+    const long long pair_tiles = P.tiles_m * ((N + 255) / 256);
     P.tiles = static_cast<int>(pair_tiles);
     const int pairs = pair_tiles < num_sms / 2 ? P.tiles : num_sms / 2;
     cudaError_t e = block == 16 ? launch_pair<16>(P, 2 * pairs, a.dtype, steps, st)
                                  : launch_pair<32>(P, 2 * pairs, a.dtype, steps, st);
     return e == cudaSuccess ? 0 : -8;
   }
-  const unsigned grid = static_cast<unsigned>(static_cast<long long>(P.tiles_m) * ((N + F_BN - 1) / F_BN) * P.splits);
+  const unsigned grid = static_cast<unsigned>(P.tiles_m * ((N + F_BN - 1) / F_BN) * P.splits);
   cudaError_t e;
 #define FX_G(BM, DEEP)                                                      \
   e = block == 16 ? launch_one<BM, 16, DEEP>(P, grid, a.dtype, steps, st) \

@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_quantize_kernel(const void *__r
 }
 
 int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda_fp4 &q, cudaStream_t st) {
-  const int col_tiles = (q.cols + Q_COLS - 1) / Q_COLS;
+  const int col_tiles = static_cast<int>((q.cols + (Q_COLS - 1LL)) / Q_COLS);
   const long long blocks = fp4_row_tiles(q.rows) * 4 * col_tiles;
   const int size = dtype == FLUX_CUDA_F32 ? 4 : 2;
   const bool vec = !(reinterpret_cast<uintptr_t>(x) & 31) && !((ldx * size) & 31);
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(Q_THREADS) fp4_dequantize_kernel(const uint8_t
 }
 
 int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long long ld, int *sat, cudaStream_t st) {
-  const int col_tiles = (q.cols + Q_COLS - 1) / Q_COLS;
+  const int col_tiles = static_cast<int>((q.cols + (Q_COLS - 1LL)) / Q_COLS);
   const long long blocks = fp4_row_tiles(q.rows) * 4 * col_tiles;
   const int size = dtype == FLUX_CUDA_F32 ? 4 : 2;
   const bool vec = !(reinterpret_cast<uintptr_t>(out) & 31) && !((ld * size) & 31);

@@ -242,3 +242,51 @@ def test_dequantize_next_to_ties(fx, ctx, name, fmt):
         m = Matrix(fx, 4, 64, fmt, s, ref.pack(code, byte))
         want = _round_once(ref.values(code, byte, fmt, s), name)
         assert (_read_back(fx, ctx, m, 4, 64, name, 0) == want).all()
+
+
+# ---------------------------------------------------------------------------------------------------- the largest sizes
+@pytest.mark.parametrize("fmt", [16, 32])
+def test_rows_as_long_as_an_int_allows(fx, ctx, fmt):
+    """One row of 2^31 - 7 columns: rounding that up to tiles takes more than 31 bits. Its last columns come out as they do
+    alone."""
+    cols, start = 2 ** 31 - 7, 2 ** 31 - 1024
+    x = torch.ones(1, cols, dtype=torch.bfloat16, device="cuda")
+    x[0, start:] = torch.randn(cols - start, device="cuda").bfloat16()
+    nc, ns = fx.fp4_bytes(1, cols, fmt)
+    codes, scales = torch.empty(nc, dtype=torch.uint8, device="cuda"), torch.empty(ns, dtype=torch.uint8, device="cuda")
+    q = fx.Fp4(codes.data_ptr(), scales.data_ptr(), 1, cols, fmt, 1.0)
+    tail = Matrix(fx, 1, cols - start, fmt)
+    alone = torch.zeros(1, cols - start, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp4_quantize(x.data_ptr(), fx.BF16, cols, q)
+    ctx.fp4_quantize(x[:, start:].data_ptr(), fx.BF16, cols - start, tail.h)
+    ctx.fp4_dequantize(tail.h, alone.data_ptr(), fx.BF16, cols - start)
+    ctx.sync()
+    assert torch.equal(codes[start // 2:], tail.codes[:tail.nc])
+    x.zero_()
+    torch.cuda.synchronize()
+    ctx.fp4_dequantize(q, x.data_ptr(), fx.BF16, cols)
+    ctx.sync()
+    one = ref.values(*ref.quantize(np.ones((1, fmt)), fmt), fmt)[0, 0]
+    assert torch.equal(x[:, start:], alone) and (x[:, :start] == one).all()
+    del x, codes, scales
+    torch.cuda.empty_cache()
+
+
+def test_as_many_rows_as_an_int_allows(fx, ctx):
+    """A product of 2^31 - 7 rows, every one of them right."""
+    rows = 2 ** 31 - 7
+    nc, ns = fx.fp4_bytes(rows, 32, 16)
+    codes = torch.full((nc,), 0x22, dtype=torch.uint8, device="cuda")  # 1
+    codes[-300 * 16:] = 0x44                                           # 2
+    scales = torch.full((ns // 4,), 0x3838, dtype=torch.int32, device="cuda")  # two blocks of factor 1, then padding
+    scales[-128:].view(32, 4)[32 - 7:, 3] = 0  # the rows past the end
+    x = fx.Fp4(codes.data_ptr(), scales.data_ptr(), rows, 32, 16, 1.0)
+    w = Matrix(fx, 1, 32, 16, 1.0, ref.pack(np.full((1, 32), 2), np.full((1, 2), 0x38, np.uint8)))
+    out = torch.zeros(rows, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemm_fp4(x, w.h, out.data_ptr(), fx.F16, 1)
+    ctx.sync()
+    assert (out[:-300] == 32).all() and (out[-300:] == 64).all()
+    del codes, scales, out
+    torch.cuda.empty_cache()
