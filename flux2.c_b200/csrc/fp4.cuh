@@ -32,7 +32,8 @@ struct Fp4GemmArgs {
   long long ld_residual;
 };
 
-// All return 0, or -8 for a failed launch / -4 for a tensor map the driver refuses.
+// All return 0, the cudaError_t (above 0) of the launch, or FP4_ERR_MAP for a tensor map the driver refuses.
+static constexpr int FP4_ERR_MAP = -4;
 int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda_fp4 &q, cudaStream_t st);
 int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long long ld, int *sat, cudaStream_t st);
 int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cudaStream_t st);

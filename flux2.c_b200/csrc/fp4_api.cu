@@ -60,7 +60,12 @@ bool too_large(const flux_cuda_fp4 &q) { return fp4_row_tiles(q.rows) * 4 * ((q.
 
 int finish(const char *op, int rc) {
   if (rc == 0) return FLUX_CUDA_OK;
-  set_error("%s: %s: %s", op, rc == -4 ? "tensor map refused" : "launch failed", cudaGetErrorString(cudaGetLastError()));
+  if (rc == FP4_ERR_MAP) {
+    set_error("%s: tensor map refused", op);
+  } else {
+    set_error("%s: launch failed: %s", op, cudaGetErrorString(static_cast<cudaError_t>(rc)));
+    cudaGetLastError();  // it has been reported
+  }
   return FLUX_CUDA_ERR_CUDA;
 }
 

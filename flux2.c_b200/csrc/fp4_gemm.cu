@@ -680,7 +680,7 @@ static int map_codes(CUtensorMap *m, const flux_cuda_fp4 &q, uint32_t box_rows) 
   CUresult r = g_encode4(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q.codes, dims, strides, box, one,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : -4;
+  return r == CUDA_SUCCESS ? 0 : FP4_ERR_MAP;
 }
 // Its factor tiles, in boxes of `chunks` tiles of one group of 128 rows (or `row_tiles` such groups).
 static int map_factors(CUtensorMap *m, const flux_cuda_fp4 &q, uint32_t chunks, uint32_t row_tiles) {
@@ -691,7 +691,7 @@ static int map_factors(CUtensorMap *m, const flux_cuda_fp4 &q, uint32_t chunks, 
   CUresult r = g_encode4(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, q.scales, dims, strides, box, one,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : -4;
+  return r == CUDA_SUCCESS ? 0 : FP4_ERR_MAP;
 }
 
 template <int BM, int BLOCK, bool DEEP, bool STEPS>
@@ -791,7 +791,7 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
   const uint32_t chunks = 256 / (4 * block);
   if (map_codes(&P.tm_w, a.w, F_BN) || map_codes(&P.tm_x, a.x, pair ? 128 : bm) || map_factors(&P.tm_ws, a.w, chunks, 1) ||
       map_factors(&P.tm_xs, a.x, chunks, pair ? 2 : 1))
-    return -4;
+    return FP4_ERR_MAP;
   P.M = a.x.rows;
   P.N = a.w.rows;
   P.slices = slices;
@@ -812,7 +812,7 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
     const int pairs = pair_tiles < num_sms / 2 ? P.tiles : num_sms / 2;
     cudaError_t e = block == 16 ? launch_pair<16>(P, 2 * pairs, a.dtype, steps, st)
                                  : launch_pair<32>(P, 2 * pairs, a.dtype, steps, st);
-    return e == cudaSuccess ? 0 : -8;
+    return e;
   }
   const unsigned grid = static_cast<unsigned>(P.tiles_m * ((N + F_BN - 1) / F_BN) * P.splits);
   cudaError_t e;
@@ -826,7 +826,7 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
   else if (bm == 64) FX_G(64, false);
   else FX_G(128, false);
 #undef FX_G
-  return e == cudaSuccess ? 0 : -8;
+  return e;
 }
 
 }  // namespace fx

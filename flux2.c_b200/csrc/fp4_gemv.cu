@@ -500,7 +500,7 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
     else FX_V(4, 3);
   }
 #undef FX_V
-  return e == cudaSuccess ? 0 : -8;
+  return e;
 }
 
 }  // namespace fx

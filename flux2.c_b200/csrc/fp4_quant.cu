@@ -17,6 +17,7 @@
 #include <math.h>
 
 #include "fp4.cuh"
+#include "launch.cuh"
 
 namespace fx {
 
@@ -247,9 +248,11 @@ int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda
   uint8_t *codes = static_cast<uint8_t *>(q.codes), *scales = static_cast<uint8_t *>(q.scales);
   const long long pitch = fp4_pitch(q.cols), chunks = fp4_chunks(q.cols, q.format);
   const float inv = 1.0f / q.scale;
-#define FX_Q(DT, BL, AL)                                                                                       \
-  fp4_quantize_kernel<DT, BL, AL><<<static_cast<unsigned>(blocks), Q_THREADS, 0, st>>>(x, ldx, q.rows, q.cols, inv, codes, \
-                                                                                       pitch, scales, chunks, col_tiles)
+  PdlOff no_overlap;  // the kernels do not wait for a predecessor themselves
+  const dim3 grid(static_cast<unsigned>(blocks)), threads(Q_THREADS);
+  cudaError_t e;
+#define FX_Q(DT, BL, AL) \
+  e = launch_kernel(fp4_quantize_kernel<DT, BL, AL>, grid, threads, 0, st, 1, x, ldx, q.rows, q.cols, inv, codes, pitch, scales, chunks, col_tiles)
 #define FX_Q2(DT)                                  \
   do {                                             \
     if (q.format == 16) {                          \
@@ -265,7 +268,7 @@ int launch_fp4_quantize(const void *x, int dtype, long long ldx, const flux_cuda
   else FX_Q2(FLUX_CUDA_BF16);
 #undef FX_Q2
 #undef FX_Q
-  return cudaGetLastError() == cudaSuccess ? 0 : -8;
+  return e;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -447,9 +450,12 @@ int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long lon
     S.mant = 2.0f * frexpf(q.scale, &S.exp), --S.exp;
     plain = fabsf(S.mant) == 1.0f && S.exp >= -126;
   }
-#define FX_D(DT, BL, AL, PL)                                                                             \
-  fp4_dequantize_kernel<DT, BL, AL, PL><<<static_cast<unsigned>(blocks), Q_THREADS, 0, st>>>(           \
-      codes, pitch, scales, chunks, q.rows, q.cols, S, out, ld, col_tiles, sat)
+  PdlOff no_overlap;
+  const dim3 grid(static_cast<unsigned>(blocks)), threads(Q_THREADS);
+  cudaError_t e;
+#define FX_D(DT, BL, AL, PL)                                                                                                 \
+  e = launch_kernel(fp4_dequantize_kernel<DT, BL, AL, PL>, grid, threads, 0, st, 1, codes, pitch, scales, chunks, q.rows, q.cols, S, \
+                    out, ld, col_tiles, sat)
 #define FX_D1(DT, BL, AL)            \
   do {                               \
     if (plain) FX_D(DT, BL, AL, true); \
@@ -471,7 +477,7 @@ int launch_fp4_dequantize(const flux_cuda_fp4 &q, void *out, int dtype, long lon
 #undef FX_D2
 #undef FX_D1
 #undef FX_D
-  return cudaGetLastError() == cudaSuccess ? 0 : -8;
+  return e;
 }
 
 }  // namespace fx

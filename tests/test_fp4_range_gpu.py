@@ -290,3 +290,58 @@ def test_as_many_rows_as_an_int_allows(fx, ctx):
     assert (out[:-300] == 32).all() and (out[-300:] == 64).all()
     del codes, scales, out
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------------------------- errors
+def test_an_earlier_error_of_the_thread_is_not_a_failed_launch(fx, ctx):
+    """A refused runtime call of the program's own (here: a device that does not exist) leaves an error that the next reader
+    gets. The operators' launches answer for themselves."""
+    import ctypes
+    runtime = ctypes.CDLL("libcudart.so.12")
+    x = torch.ones(4, 64, device="cuda")
+    q, out = Matrix(fx, 4, 64, 16), torch.zeros(4, 64, device="cuda")
+    torch.cuda.synchronize()
+    try:
+        for call in (lambda: ctx.fp4_quantize(x.data_ptr(), fx.F32, 64, q.h),
+                     lambda: ctx.fp4_dequantize(q.h, out.data_ptr(), fx.F32, 64),
+                     lambda: ctx.gemm_fp4(q.h, q.h, out.data_ptr(), fx.F32, 64),
+                     lambda: ctx.gemv_fp4(x.data_ptr(), fx.F32, 64, 4, q.h, out.data_ptr(), fx.F32, 64)):
+            assert runtime.cudaSetDevice(10 ** 6) != 0
+            call()
+            assert runtime.cudaGetLastError() != 0  # and it is still there for its own reader
+    finally:
+        runtime.cudaGetLastError()
+    ctx.sync()
+
+
+def test_a_failed_launch_names_its_cause(fx, ctx):
+    """Launches into a capture that the program has spoilt (by waiting for the stream inside of it) are refused by the runtime,
+    and the refusal's own text comes back; afterwards everything works as before."""
+    import ctypes
+    runtime = ctypes.CDLL("libcudart.so.12")
+    runtime.cudaGetErrorString.restype = ctypes.c_char_p
+    x = torch.ones(4, 64, device="cuda")
+    q, out = Matrix(fx, 4, 64, 16), torch.zeros(4, 64, device="cuda")
+    few = torch.zeros(4, 4, device="cuda")
+    calls = (lambda: ctx.fp4_quantize(x.data_ptr(), fx.F32, 64, q.h),
+             lambda: ctx.fp4_dequantize(q.h, out.data_ptr(), fx.F32, 64),
+             lambda: ctx.gemm_fp4(q.h, q.h, few.data_ptr(), fx.F32, 4),
+             lambda: ctx.gemv_fp4(x.data_ptr(), fx.F32, 64, 4, q.h, few.data_ptr(), fx.F32, 4))
+    torch.cuda.synchronize()
+    for call in calls:
+        stream, graph = ctypes.c_void_p(ctx.stream), ctypes.c_void_p()
+        assert runtime.cudaStreamBeginCapture(stream, 2) == 0
+        spoilt = runtime.cudaStreamSynchronize(stream)
+        runtime.cudaGetLastError()
+        try:
+            with pytest.raises(fx.FluxCudaError) as e:
+                call()
+        finally:
+            runtime.cudaStreamEndCapture(stream, ctypes.byref(graph))
+            runtime.cudaGetLastError()
+        assert spoilt != 0
+        assert "launch failed" in str(e.value) and runtime.cudaGetErrorString(901).decode() in str(e.value)
+    for call in calls:
+        call()
+    ctx.sync()
+    assert (few == 64 * ref.values(*ref.quantize(np.ones((1, 64)), 16), 16)[0, 0]).all()  # ones are 6 * e4m3(1 / 6)
