@@ -186,9 +186,10 @@ def _round_once(v, name):
     p, low, top = {"f32": (24, -126, F32_MAX), "f16": (11, -14, 65504.0),
                    "bf16": (8, -126, float(torch.finfo(torch.bfloat16).max))}[name]
     e = np.maximum(np.frexp(v)[1] - 1, low).astype(np.float64)
-    step = np.exp2(e - (p - 1))
-    r = np.round(v / step) * step
-    return np.where(np.abs(r) > top, np.sign(r) * (65504.0 if name == "f16" else np.inf), r)
+    with np.errstate(invalid="ignore", over="ignore"):
+        step = np.exp2(e - (p - 1))
+        r = np.round(v / step) * step
+    return np.where(np.abs(r) > top, np.copysign(65504.0 if name == "f16" else np.inf, v), r)
 
 
 def _scales_next_to_ties():
@@ -345,3 +346,120 @@ def test_a_failed_launch_names_its_cause(fx, ctx):
         call()
     ctx.sync()
     assert (few == 64 * ref.values(*ref.quantize(np.ones((1, 64)), 16), 16)[0, 0]).all()  # ones are 6 * e4m3(1 / 6)
+
+
+# ---------------------------------------------------------------------------------------------------- sums known to the bit
+def _sparse(rng, rows, cols, fmt):
+    """Codes +-1 with factor 1 and a value per row and column: a lost or doubled column changes every sum."""
+    code = rng.choice([2, 10], (rows, cols))
+    byte = np.full((rows, -(-cols // fmt)), 127 if fmt == 32 else 0x38, np.uint8)
+    return code, byte
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+@pytest.mark.parametrize("xname", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,K", [(1, 60000), (3, 20000), (16, 30000), (1, 65536), (5, 65536), (7, 9216), (16, 9216), (2, 65505)])
+def test_few_row_product_of_long_rows_to_the_bit(fx, ctx, M, K, xname, fmt):
+    """Whole numbers of at most 7 bits times +-1: every partial sum is an exact f32 number (below 2^24), so the result is
+    exact however the sum is split, and no column may be lost or counted twice."""
+    rng = np.random.default_rng(K + M)
+    code, byte = _sparse(rng, 40, K, fmt)
+    w, wv = Matrix(fx, 40, K, fmt, 1.0, ref.pack(code, byte)), ref.values(code, byte, fmt)
+    dev, x = _plain(rng.integers(1, 128, (M, K)).astype(np.float64), xname, K)
+    out = torch.zeros(M, 40, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemv_fp4(dev.data_ptr(), _dt(fx, xname), K, M, w.h, out.data_ptr(), fx.F32, 40)
+    ctx.sync()
+    assert (out.double().cpu().numpy() == x @ wv.T).all()
+
+
+@pytest.mark.parametrize("M,K", [(1, 60000), (3, 20000), (1, 65536), (5, 65536), (4, 9216)])
+def test_few_row_product_adds_short_chains(fx, ctx, M, K):
+    """The tensor instruction may truncate, the additions of its chains round. All numbers are positive, so that truncation
+    adds up and no cancellation widens the bound. A chain is 128 columns, 8 instructions for each part of x, an instruction
+    truncates what it has added up and its aligned products: 2 * 2^-23 of the chain each. The chains and the pieces of a
+    sum (40 at most: 16 warps twice, 8 CTAs) are added with n = K / 128 + 40 roundings of at most 2^-24 of the sum either way;
+    6 sqrt(n) of those are exceeded once in 10^7 (Hoeffding)."""
+    rng = np.random.default_rng(K)
+    code, byte = ref.quantize(np.abs(rng.standard_normal((40, K))), 16)
+    w, wv = Matrix(fx, 40, K, 16, 1.0, ref.pack(code, byte)), ref.values(code, byte, 16)
+    dev, x = _plain(np.abs(rng.standard_normal((M, K))), "f32", K)
+    out = torch.zeros(M, 40, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemv_fp4(dev.data_ptr(), fx.F32, K, M, w.h, out.data_ptr(), fx.F32, 40)
+    ctx.sync()
+    want = x @ wv.T
+    tol = want * (8 * 2 * 2.0 ** -23 + 6 * np.sqrt(K / 128 + 40) * 2.0 ** -24)
+    assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+@pytest.mark.parametrize("M,N,K", [(1, 130, 60000), (20, 200, 9000), (40, 140, 20001), (100, 260, 9216), (130, 300, 5000),
+                                   (300, 500, 9999), (1025, 2049, 1600), (1300, 2200, 300), (16, 20000, 600), (2600, 5200, 64)])
+def test_product_to_the_bit(fx, ctx, M, N, K, fmt):
+    """Codes under factors 1 and 2: sums of at most 2^24 quarters are exact f32 numbers, so the result is exact however the sum is
+    split, and every block needs its own factor."""
+    rng = np.random.default_rng(M + N + K)
+
+    def matrix(rows):
+        code = rng.choice([0, 1, 2, 9, 10, 3, 11], (rows, K))  # 0, +-0.5, +-1, +-1.5
+        byte = rng.choice([127, 128] if fmt == 32 else [0x38, 0x40], (rows, -(-K // fmt))).astype(np.uint8)
+        return Matrix(fx, rows, K, fmt, 1.0, ref.pack(code, byte)), ref.values(code, byte, fmt)
+
+    x, xv = matrix(M)
+    w, wv = matrix(N)
+    assert (np.abs(xv).sum(1) * 3).max() < 2 ** 22
+    out = torch.zeros(M, N, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemm_fp4(x.h, w.h, out.data_ptr(), fx.F32, N)
+    ctx.sync()
+    want = (torch.from_numpy(xv).cuda() @ torch.from_numpy(wv).cuda().T).cpu().numpy()
+    assert (out.double().cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+@pytest.mark.parametrize("side", ["w", "x"])
+@pytest.mark.parametrize("M,K", [(16, 32), (128, 32), (200, 300)])
+def test_product_with_every_factor(fx, ctx, M, K, side, fmt):
+    """Every finite factor with every code on the tensor cores, against rows that pick out one column each: single exact products.
+    Results below the normal range may be lost (2^-126 in all); what lies beyond the f32 range is left out; NaN stays in its row."""
+    code = np.tile(np.arange(16), (256, -(-K // 16)))[:, :K]
+    byte = np.repeat(np.arange(256)[:, None], -(-K // fmt), 1).astype(np.uint8)
+    if fmt == 16:
+        byte &= 127
+    every, ev = Matrix(fx, 256, K, fmt, 1.0, ref.pack(code, byte)), ref.values(code, byte, fmt)
+    at = np.arange(M) * 7 % K
+    pcode = np.zeros((M, K), np.int64)
+    pcode[np.arange(M), at] = 2
+    pbyte = np.full((M, -(-K // fmt)), 127 if fmt == 32 else 0x38, np.uint8)
+    pick = Matrix(fx, M, K, fmt, 1.0, ref.pack(pcode, pbyte))
+    out = torch.zeros((M, 256) if side == "w" else (256, M), device="cuda")
+    torch.cuda.synchronize()
+    if side == "w":
+        ctx.gemm_fp4(pick.h, every.h, out.data_ptr(), fx.F32, 256)
+    else:
+        ctx.gemm_fp4(every.h, pick.h, out.data_ptr(), fx.F32, M)
+    ctx.sync()
+    got = out.double().cpu().numpy()
+    got = got if side == "w" else got.T
+    want = ev[:, at].T
+    inside = np.isnan(ev).any(1) | (np.abs(ev).max(1) < F32_MAX)
+    assert inside.sum() >= 252
+    assert (np.isnan(got) == np.isnan(want))[:, inside].all()
+    fine = np.broadcast_to(inside, want.shape) & np.isfinite(want)
+    small = fine & (np.abs(want) < 2.0 ** -126)
+    assert (got == want)[fine & ~small].all()
+    assert (np.abs(got - want)[small] <= 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("e", [-125, -100, -60, -1, 0, 1, 60, 100, 125])
+def test_product_of_opposite_factors(fx, ctx, e):
+    """2^e against 2^-e: products near 1, however far the factors are from it."""
+    rng = np.random.default_rng(e + 200)
+    x, xv = _exact_matrix(fx, rng, 20, 512, 32, e, 1.0)
+    w, wv = _exact_matrix(fx, rng, 140, 512, 32, -e, 1.0)
+    out = torch.zeros(20, 140, device="cuda")
+    torch.cuda.synchronize()
+    ctx.gemm_fp4(x.h, w.h, out.data_ptr(), fx.F32, 140)
+    ctx.sync()
+    assert (out.double().cpu().numpy() == xv @ wv.T).all()
