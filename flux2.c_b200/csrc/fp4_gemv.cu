@@ -457,11 +457,11 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
   P.kparts = 1;
   while (P.kparts < 8 && P.kparts * 2 <= P.steps && x_bytes(P.group, P.kparts) > V_SMEM_MAX - sums_room * (1 + (P.group > 4))) P.kparts *= 2;
   while (P.group > 1 && x_bytes(P.group, P.kparts) + (2 * V_WARPS + 1) * 128LL * P.group > V_SMEM_MAX) P.group = (P.group + 1) / 2;
-  const int groups = (rows + P.group - 1) / P.group;
+  const int sets = (rows + P.group - 1) / P.group;
   // Of the ways to split K further, as long as a warp gets a step, the one that ends first: clusters at once, and how evenly
   // the units go into them.
   auto held = [&](int kparts) {
-    const long long n = g_clusters[device][kparts == 1 ? 0 : kparts == 2 ? 1 : kparts == 4 ? 2 : 3] / groups;
+    const long long n = g_clusters[device][kparts == 1 ? 0 : kparts == 2 ? 1 : kparts == 4 ? 2 : 3] / sets;
     return n < 1 ? 1 : n > P.units ? P.units : n;
   };
   // in steps of a warp: what the busiest cluster's warps do, a quarter for joining parts, and laying out x (a fifth of a
@@ -474,11 +474,39 @@ int launch_gemv_fp4(const void *x, int x_dtype, long long ldx, int rows, const f
   for (int k = P.kparts * 2, i = P.kparts == 1 ? 1 : P.kparts == 2 ? 2 : 3; k <= 8 && k <= P.steps; k *= 2, ++i)
     if (g_clusters[device][i] > 0 && longest(k) < longest(split)) split = k;
   P.kparts = split;
+  // What a choice comes to: the sums of a cluster's units lie next to x, so where x leaves little room there are more clusters
+  // than the device holds at once, in rounds that lay out x again.
+  struct Plan {
+    long long clusters, rounds;
+    double time;  // in steps of a warp and 8 columns, as above, with what a round costs at the least
+  };
+  auto plan = [&](int group, int kparts) {
+    const int sets = (rows + group - 1) / group, i = kparts == 1 ? 0 : kparts == 2 ? 1 : kparts == 4 ? 2 : 3;
+    const long long x = x_bytes(group, kparts), room = (V_SMEM_MAX - x) / (128LL * group) - 2 * V_WARPS;
+    const long long at_once = g_clusters[device][i] < 1 ? 1 : g_clusters[device][i];
+    Plan p;
+    p.clusters = at_once / sets < 1 ? 1 : at_once / sets > P.units ? P.units : at_once / sets;
+    if (P.units > p.clusters * room) p.clusters = (P.units + room - 1) / room;
+    p.rounds = (p.clusters * sets + at_once - 1) / at_once;
+    const long long pairs = (P.units + p.clusters - 1) / p.clusters * ((P.steps + kparts - 1) / kparts);
+    const double step[4] = {1.0, 1.3, 1.6, 1.7};  // of 8, 16, 24 and 32 columns
+    p.time = p.rounds * (0.5 + pairs * step[(group * parts - 1) / 8] / V_WARPS + 0.4 * x / (16 * V_THREADS) + 0.25 * (kparts > 1));
+    return p;
+  };
+  Plan chosen = plan(P.group, P.kparts);
+  // Several rounds: the least of all choices that fit. (18432 x 9216: 7 f32 rows 309 -> 93 us as four sets of two, 12 bf16 rows
+  // 225 -> 63, 16 f16 rows of 19456 x 2560: 55 -> 37; over 24 such sizes the choice is within a tenth of the best one.)
+  if (chosen.rounds > 1) {
+    for (int group = 1; group <= rows && group * parts <= 32; ++group)
+      for (int kparts = 1, i = 0; kparts <= 8 && kparts <= P.steps; kparts *= 2, ++i) {
+        if (g_clusters[device][i] < 1 || x_bytes(group, kparts) + (2 * V_WARPS + 1) * 128LL * group > V_SMEM_MAX) continue;
+        const Plan p = plan(group, kparts);
+        if (p.time < chosen.time) chosen = p, P.group = group, P.kparts = kparts;
+      }
+  }
+  const int groups = (rows + P.group - 1) / P.group;
+  const long long clusters = chosen.clusters;
   P.part_steps = (P.steps + P.kparts - 1) / P.kparts;
-  long long clusters = held(P.kparts);
-  // the sums of a cluster's units next to x
-  const long long room = (V_SMEM_MAX - x_bytes(P.group, P.kparts)) / (128LL * P.group) - 2 * V_WARPS;
-  if (P.units > clusters * room) clusters = (P.units + room - 1) / room;
   P.clusters = static_cast<int>(clusters);
   const size_t smem = static_cast<size_t>(V_RING + x_bytes(P.group, P.kparts) +
                                           ((P.units + clusters - 1) / clusters + 2 * V_WARPS) * 128 * P.group);

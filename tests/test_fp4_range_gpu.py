@@ -463,3 +463,73 @@ def test_product_of_opposite_factors(fx, ctx, e):
     ctx.gemm_fp4(x.h, w.h, out.data_ptr(), fx.F32, 140)
     ctx.sync()
     assert (out.double().cpu().numpy() == xv @ wv.T).all()
+
+
+# ---------------------------------------------------------------------------------------------------- five rows and more
+def _weights_of_ones(fx, N, K, fmt):
+    """+-1 with factors 1 and 2, made on the device, and its values in 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(N + K)
+    sign = torch.randint(0, 2, (N, K), device="cuda", generator=g, dtype=torch.uint8)
+    code = torch.zeros(N, 32 * -(-K // 32), dtype=torch.uint8, device="cuda")
+    code[:, :K] = 2 | sign << 3
+    up = torch.randint(0, 2, (N, -(-K // fmt)), device="cuda", generator=g, dtype=torch.uint8)
+    m = Matrix(fx, N, K, fmt)
+    m.codes[:m.nc] = (code[:, 0::2] | code[:, 1::2] << 4).reshape(-1)
+    byte = (127 + up) if fmt == 32 else (0x38 + 8 * up)
+    tiles, chunks = -(-N // 128), -(-up.shape[1] // 4)
+    full = torch.zeros(tiles * 128, chunks * 4, dtype=torch.uint8, device="cuda")
+    full[:N, :up.shape[1]] = byte
+    m.scales[:m.ns] = full.view(tiles, 4, 32, chunks, 4).permute(0, 3, 2, 1, 4).reshape(-1)
+    values = (1.0 - 2.0 * sign.double()) * (1.0 + up.double()).repeat_interleave(fmt, 1)[:, :K]
+    return m, values
+
+
+@pytest.mark.parametrize("fmt", [16, 32])
+@pytest.mark.parametrize("N,K", [(18432, 9216), (19456, 2560), (2560, 9728), (5000, 4001)])
+def test_few_row_product_of_every_number_of_rows(fx, ctx, N, K, fmt):
+    """Every number of rows and type, so every way to lay them out: sets of rows, splits of K, several rounds of clusters. Whole
+    numbers of a sum of magnitudes below 2^24: exact."""
+    w, wv = _weights_of_ones(fx, N, K, fmt)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    for name in ("bf16", "f16", "f32"):
+        for m in range(1, 17):
+            x = torch.randint(-127, 128, (m, K), device="cuda", generator=g).to(TORCH[name])
+            out = torch.full((m + 1, N), 7.0, device="cuda")
+            torch.cuda.synchronize()
+            ctx.gemv_fp4(x.data_ptr(), _dt(fx, name), K, m, w.h, out.data_ptr(), fx.F32, N)
+            ctx.sync()
+            assert (out[:m].double() == x.double() @ wv.T).all() and (out[m:] == 7).all(), (name, m)
+
+
+@pytest.mark.parametrize("N,K", [(18432, 9216), (19456, 2560), (9728, 2560), (2560, 9728)])
+def test_more_rows_cost_no_more_than_calls_of_four(fx, ctx, N, K):
+    """One call of 5 to 16 rows is not slower than as many calls of four rows as they make (a quarter is allowed for noise).
+    Weights of more than the caches hold are gone through in turn."""
+    sets = max(2, int(3e8 / (0.56 * N * K)))
+    ws = [Matrix(fx, N, K, 16) for _ in range(sets)]
+    for w in ws:
+        w.codes[:w.nc] = 0x22
+        w.scales[:w.ns] = 0x38
+    x = torch.ones(16, K, device="cuda")
+    out = torch.zeros(16, N, device="cuda")
+    stream = torch.cuda.ExternalStream(ctx.stream)
+
+    def time(name, m):
+        xt = x.to(TORCH[name])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for w in ws:
+                ctx.gemv_fp4(xt.data_ptr(), _dt(fx, name), K, m, w.h, out.data_ptr(), fx.F32, N)
+        e = [torch.cuda.Event(enable_timing=True) for _ in range(8)]
+        with torch.cuda.stream(stream):
+            for ev in e:
+                graph.replay()
+                ev.record(stream)
+        torch.cuda.synchronize()
+        return min(a.elapsed_time(b) for a, b in zip(e, e[1:]))
+
+    for name in ("bf16", "f16", "f32"):
+        four = time(name, 4)
+        for m in range(5, 17):
+            assert time(name, m) <= 1.25 * -(-m // 4) * four, (name, m)
