@@ -44,7 +44,7 @@ def needs_build(lib=LIB):
 def build(force=False, verbose=False, checked=False):
     """Compile every source under csrc/ into libflux_cuda.so (one nvcc -c per file, then a link). checked=True builds
     libflux_cuda_debug.so instead: the same sources with -DFLUX_CUDA_DEBUG (index and alignment checks in the
-    kernels that record a violation in the context's error word instead of accessing memory)."""
+    16-bit GEMM, attention and AdaLN kernels that record a violation in the context's error word instead of accessing memory)."""
     lib = LIB_CHECKED if checked else LIB
     extra = ["-DFLUX_CUDA_DEBUG"] if checked else []
     if not force and not needs_build(lib):

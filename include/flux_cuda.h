@@ -28,8 +28,8 @@ extern "C" {
 typedef struct flux_cuda_ctx flux_cuda_ctx;
 
 const char *flux_cuda_last_error(void);
-/* 1 for the checked build of the library (compiled with -DFLUX_CUDA_DEBUG: libflux_cuda_debug.so), whose kernels verify
- * the tile, row and alignment arithmetic of what they are about to access and, on a violation, record it in the
+/* 1 for the checked build of the library (compiled with -DFLUX_CUDA_DEBUG: libflux_cuda_debug.so), whose 16-bit GEMM,
+ * attention and AdaLN kernels verify the tile, row and alignment arithmetic of what they are about to access and, on a violation, record it in the
  * context's error word (reported as FLUX_CUDA_ERR_KERNEL by the next synchronising call) and skip the access - they
  * never trap. 0 for the normal build. The reference's counterpart is its -fsanitize=address debug target. */
 int flux_cuda_build_checked(void);
@@ -464,8 +464,9 @@ int flux_cuda_qk_norm_rope(flux_cuda_ctx *ctx, void *qkv, long long ld, int q_co
  *         ((r / 128) * ceil(blocks / 4) + b / 4) * 512, byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of it (the order
  *         the tensor cores take); rows and blocks past the end hold 0.
  * flux_cuda_fp4_quantize writes both, padding included; matrices from elsewhere must keep to it, and for the products hold
- * no code * factor beyond the f32 range (MXFP4 factors above 2^125; the rows that do hold them come out unspecified). Both 16-byte aligned;
- * rows [128 i, ...) of a matrix are a matrix of their own (codes + 128 i * row bytes, scales + i * ceil(blocks / 4) * 512).
+ * no code * factor beyond the f32 range (MXFP4 factors above 2^125; the rows that do hold them come out unspecified).
+ * Both 16-byte aligned; rows [128 i, ...) of a matrix are a matrix of their own (codes + 128 i * row bytes, scales + i *
+ * ceil(blocks / 4) * 512). No call's output may overlap an input, but for the residual of flux_cuda_gemm_fp4.
  * ---------------------------------------------------------------------------------------------- */
 #define FLUX_CUDA_NVFP4 16 /* blocks of 16 columns, factor e4m3 without a sign (bytes 0 .. 0x7E, at most 448; 0x7F is NaN) */
 #define FLUX_CUDA_MXFP4 32 /* blocks of 32 columns, factor 2^(byte - 127) (0xFF is NaN) */
@@ -494,9 +495,9 @@ int flux_cuda_fp4_dequantize(flux_cuda_ctx *ctx, const flux_cuda_fp4 *q, void *o
  * out[m, n] = residual[m, n] + gate[n] * sum_k x[m, k] w[n, k] on the block-scaled tensor-core path: the 4-bit form of
  * flux_cuda_gemm_bf16's STORE and GATED_RES epilogues. x [M, K], w [N, K] of one format; any M, N >= 0, K >= 1. out of
  * `dtype` with row pitch ld_out; f32 sums of code * factor, then the two scales (whose product may lie outside f32), rounded
- * once (f16 saturates and is counted). gate f32 [N] or NULL (1);
- * residual f32 [M, N] with row pitch ld_residual, or NULL (0); it may be `out` itself in f32 with the same pitch,
- * otherwise no output may overlap an input. Row pitches are below 2^30 elements. A NaN factor makes the products of its row or column NaN.
+ * once (f16 saturates and is counted). gate f32 [N] or NULL (1); residual f32 [M, N] with row pitch ld_residual, or NULL
+ * (0); it may be `out` itself in f32 with the same pitch. Row pitches are below 2^30 elements. A NaN factor makes the
+ * products of its row or column NaN.
  */
 int flux_cuda_gemm_fp4(flux_cuda_ctx *ctx, const flux_cuda_fp4 *x, const flux_cuda_fp4 *w, void *out, int dtype,
                        long long ld_out, const float *gate, const float *residual, long long ld_residual);
