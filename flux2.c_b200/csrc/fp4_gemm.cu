@@ -35,7 +35,7 @@ struct alignas(64) Fp4GemmParams {
   int tiles_m, tiles;
   int splits;                // CTAs of a cluster that share one output tile, each with its part of the k-slices
   float alpha;               // x.scale * w.scale
-  float pre, pre2;           // STEPS: the same as two factors (fp4_alpha), and alpha is 1
+  float scale_x, scale_w;    // STEPS: the two
   void *out;
   const float *gate, *residual;
   uint32_t pitch, res_pitch;  // bytes from row to row of out and residual
@@ -127,28 +127,45 @@ __device__ __forceinline__ void fp4_residual(float (&v)[16], int rows, const uin
       v[j] = j < rows ? __ldcg(reinterpret_cast<const float *>(res + static_cast<uint64_t>(res_pitch) * j)) : 0.f;
   }
 }
-// What a sum is multiplied by. STEPS = false: a = alpha * gate in one step, for calls without a gate or with alpha = 1, and
-// alpha a normal f32. Otherwise alpha * gate (or the scales' product) may leave the f32 range although the result does not, so
-// the sum is taken to x.scale * w.scale first and to a = gate then; a gate of 0 leaves nothing of a sum of any size.
+// What the sums of column n are multiplied by: x.scale * w.scale * gate. STEPS = false: in one step, for calls whose alpha is a
+// normal f32 and that have no gate, or alpha = 1. Otherwise the product may be no normal f32 although the result is one;
+// it is then three factors that take a sum the same way, so that nothing on the way leaves f32 unless the result does.
+// (Sums are 0 or 2^-149 .. 2^128, so powers of two beyond 2^300 need not be told apart.)
 // Instances of their own, because the multiplications cost every other call 0.2 - 0.3 us of exposed epilogue, even behind a
 // branch (1024 x 6144 x 2560: 13.6 -> 13.9 us).
+struct Fp4Factor {
+  float a, pre, pre2;
+};
 template <bool STEPS>
-__device__ __forceinline__ float fp4_scaled(float sum, float a, float pre, float pre2) {
-  return STEPS ? sum * (a == 0.f ? 0.f : pre) * pre2 : sum;
+__device__ __forceinline__ Fp4Factor fp4_column(const Fp4GemmParams &P, int n) {
+  if (!STEPS) return {P.gate ? P.alpha * P.gate[n] : P.alpha, 1.0f, 1.0f};
+  const double t = static_cast<double>(P.scale_x) * P.scale_w * (P.gate ? P.gate[n] : 1.0f);
+  const float a = static_cast<float>(t);
+  if (t == 0 || !(fabs(t) < __longlong_as_double(0x7FF0000000000000LL)) || (fabsf(a) >= 1.17549435e-38f && fabsf(a) <= 3.402823466e38f))
+    return {a, 1.0f, 1.0f};
+  const long long bits = __double_as_longlong(t);
+  const double mant = __longlong_as_double((bits & 0x800FFFFFFFFFFFFFLL) | 0x3FF0000000000000LL);  // t = mant 2^e
+  const int e = min(max(static_cast<int>(bits >> 52 & 0x7FF) - 1023, -300), 300), k = e / 3;
+  const auto two = [](int i) { return __uint_as_float(static_cast<uint32_t>(i + 127) << 23); };
+  return {static_cast<float>(mant) * two(k), two(k), two(e - 2 * k)};
 }
-// Epilogue of 16 output rows of this thread's column n, starting at `out`: a = alpha * gate, v the residual if any. Each row's
+template <bool STEPS>
+__device__ __forceinline__ float fp4_scaled(float sum, float pre, float pre2) {
+  return STEPS ? sum * pre * pre2 : sum;
+}
+// Epilogue of 16 output rows of this thread's column n, starting at `out`: f from fp4_column, v the residual if any. Each row's
 // address is one multiply-add of its own (row pitches are 32 bits, checked on the host), and whole blocks carry no
 // predicates: one warp per scheduler has nothing to hide a chain of 64-bit additions or a branch behind. Checked and
 // addressed row by row a store cost 150 cycles, along a chain 32.
 template <int DT, bool STEPS>
 __device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], float (&v)[16], bool residual, int rows, uint8_t *out,
-                                         uint32_t pitch, float a, float pre, float pre2, float &mx) {
+                                         uint32_t pitch, const Fp4Factor &f, float &mx) {
   if (residual) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = fmaf(a, fp4_scaled<STEPS>(__uint_as_float(r[j]), a, pre, pre2), v[j]);
+    for (int j = 0; j < 16; ++j) v[j] = fmaf(f.a, fp4_scaled<STEPS>(__uint_as_float(r[j]), f.pre, f.pre2), v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = a * fp4_scaled<STEPS>(__uint_as_float(r[j]), a, pre, pre2);
+    for (int j = 0; j < 16; ++j) v[j] = f.a * fp4_scaled<STEPS>(__uint_as_float(r[j]), f.pre, f.pre2);
   }
   if (rows >= 16) {
     if (DT == FLUX_CUDA_F32) {
@@ -174,11 +191,11 @@ __device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], float (&v)[16]
 // used: a load from another SM takes most of a microsecond.
 template <int DT, int SP, int R, bool STEPS>
 __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m_end, int n, int N, uint8_t *out,
-                                         long long pitch, const uint8_t *res, long long res_pitch, float alpha, float pre,
-                                         float pre2, const float *gate, float &mx) {
-  float g[4];
+                                         long long pitch, const uint8_t *res, long long res_pitch,
+                                         const Fp4GemmParams &P, float &mx) {
+  Fp4Factor f[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) g[i] = gate && n + i < N ? alpha * gate[n + i] : alpha;
+  for (int i = 0; i < 4; ++i) f[i] = fp4_column<STEPS>(P, n + i < N ? n + i : N - 1);
   for (; m < m_end; m += 4 * R) {
     float4 v[SP][R];
     float y[R][4];  // the residual, all of it requested before anything is stored (it may be `out`)
@@ -202,10 +219,10 @@ __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m
 #pragma unroll
       for (int s = 1; s < SP; ++s)
         if (s < splits) a.x += v[s][j].x, a.y += v[s][j].y, a.z += v[s][j].z, a.w += v[s][j].w;
-      y[j][0] = fmaf(g[0], fp4_scaled<STEPS>(a.x, g[0], pre, pre2), y[j][0]);
-      y[j][1] = fmaf(g[1], fp4_scaled<STEPS>(a.y, g[1], pre, pre2), y[j][1]);
-      y[j][2] = fmaf(g[2], fp4_scaled<STEPS>(a.z, g[2], pre, pre2), y[j][2]);
-      y[j][3] = fmaf(g[3], fp4_scaled<STEPS>(a.w, g[3], pre, pre2), y[j][3]);
+      y[j][0] = fmaf(f[0].a, fp4_scaled<STEPS>(a.x, f[0].pre, f[0].pre2), y[j][0]);
+      y[j][1] = fmaf(f[1].a, fp4_scaled<STEPS>(a.y, f[1].pre, f[1].pre2), y[j][1]);
+      y[j][2] = fmaf(f[2].a, fp4_scaled<STEPS>(a.z, f[2].pre, f[2].pre2), y[j][2]);
+      y[j][3] = fmaf(f[3].a, fp4_scaled<STEPS>(a.w, f[3].pre, f[3].pre2), y[j][3]);
     }
 #pragma unroll
     for (int j = 0; j < R; ++j)
@@ -329,7 +346,7 @@ __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const
     const int q = warp & 3;  // the lane group of TMEM this warp may read
     const int nl = q * 32 + lane, n = n0 + nl;
     const int live = P.M - m0 < BM ? P.M - m0 : BM;
-    const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
+    const Fp4Factor f = fp4_column<STEPS>(P, n < P.N ? n : P.N - 1);
     float mx = 0.f;
     const long long pitch = P.pitch, res_pitch = P.res_pitch;
     uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * static_cast<long long>(FP4_SIZE<DT>);
@@ -356,7 +373,7 @@ __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const
         } else if (direct) {
           float next[16];
           if (res) fp4_residual(next, live - c - STEP, res + (c + STEP) * res_pitch, P.res_pitch);
-          fp4_emit<DT, STEPS>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, P.pre, P.pre2, mx);
+          fp4_emit<DT, STEPS>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, f, mx);
           if (res) {
 #pragma unroll
             for (int j = 0; j < STEP; ++j) v[j] = next[j];
@@ -373,9 +390,9 @@ __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const
         const uint32_t mine = smem_u32(part) + lane * 16;
         uint8_t *o = static_cast<uint8_t *>(P.out) + m0 * pitch + nj * static_cast<long long>(FP4_SIZE<DT>);
         const uint8_t *r = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + nj * 4LL : nullptr;
-        if (P.splits <= 2) fp4_join<DT, 2, 8, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.pre, P.pre2, P.gate, mx);
-        else if (P.splits <= 4) fp4_join<DT, 4, 4, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.pre, P.pre2, P.gate, mx);
-        else fp4_join<DT, 8, 2, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P.alpha, P.pre, P.pre2, P.gate, mx);
+        if (P.splits <= 2) fp4_join<DT, 2, 8, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, mx);
+        else if (P.splits <= 4) fp4_join<DT, 4, 4, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, mx);
+        else fp4_join<DT, 8, 2, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, mx);
       }
     }
     sat_report(P.err + 1, DT == FLUX_CUDA_F16, mx);
@@ -537,7 +554,7 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
     for (int tile = pair; tile < P.tiles; tile += num_pairs, ++t) {
       const int m0 = (tile % P.tiles_m) * 256, n = (tile / P.tiles_m) * 256 + static_cast<int>(rank) * 128 + q * 32 + lane;
       const int live = n < P.N ? (P.M - m0 < 256 ? P.M - m0 : 256) : 0;
-      const float a = P.gate && n < P.N ? P.alpha * P.gate[n] : P.alpha;
+      const Fp4Factor f = fp4_column<STEPS>(P, n < P.N ? n : P.N - 1);
       const uint32_t acc = tmem + (t & 1) * C::ACC1 + (static_cast<uint32_t>(q * 32) << 16);
       const long long pitch = P.pitch, res_pitch = P.res_pitch;
       uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * static_cast<long long>(FP4_SIZE<DT>);
@@ -552,7 +569,7 @@ __global__ void __launch_bounds__(F2_THREADS, 1) gemm2_fp4_kernel(const __grid_c
       float v0[16], v1[16];
       auto column = [&](int i) { return (shared + 16 * (2 * i + half)) & 255; };
       auto finish = [&](const uint32_t (&r)[16], float (&v)[16], int c) {
-        fp4_emit<DT, STEPS>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, a, P.pre, P.pre2, mx);
+        fp4_emit<DT, STEPS>(r, v, res != nullptr, live - c, out + c * pitch, P.pitch, f, mx);
       };
       auto fetch = [&](float (&v)[16], int c) {
         if (res) fp4_residual(v, live - c, res + c * res_pitch, P.res_pitch);
@@ -764,21 +781,6 @@ static Fp4Choice fp4_choose(long long M, long long N, int slices, long long pitc
   return best;
 }
 
-// The two scales as factors that a sum is multiplied by one after the other: their product and 1, or, where f32 has no normal
-// number for the product, two that take the sum the same way, so that it leaves the f32 range only if the result does.
-static void fp4_alpha(float x, float w, float &first, float &second) {
-  const double both = static_cast<double>(x) * w;  // exact
-  first = static_cast<float>(both), second = 1.0f;
-  if (both == 0 || (fabsf(first) >= FLT_MIN && fabsf(first) <= FLT_MAX)) return;
-  if ((fabsf(x) >= 1.0f) == (fabsf(w) >= 1.0f)) {
-    first = x, second = w;
-  } else {  // a subnormal scale against one that is at least 1
-    int e;
-    const double m = frexp(both, &e);
-    first = ldexpf(static_cast<float>(m), e / 2), second = ldexpf(1.0f, e - e / 2);
-  }
-}
-
 int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cudaStream_t st) {
   Fp4GemmParams P;
   memset(&P, 0, sizeof(P));
@@ -797,9 +799,11 @@ int launch_gemm_fp4(const Fp4GemmArgs &a, int device, int num_sms, int *err, cud
   P.slices = slices;
   P.tiles_m = static_cast<int>((M + bm - 1) / bm);
   P.splits = choice.splits;
-  fp4_alpha(a.x.scale, a.w.scale, P.pre, P.pre2);
-  const bool steps = P.pre2 != 1.0f || (a.gate && P.pre != 1.0f);
-  P.alpha = steps ? 1.0f : P.pre;
+  P.alpha = a.x.scale * a.w.scale;
+  P.scale_x = a.x.scale;
+  P.scale_w = a.w.scale;
+  const bool normal = (fabsf(P.alpha) >= FLT_MIN && fabsf(P.alpha) <= FLT_MAX) || a.x.scale == 0 || a.w.scale == 0;
+  const bool steps = !normal || (a.gate && P.alpha != 1.0f);
   P.out = a.out;
   P.pitch = static_cast<uint32_t>(a.ld_out * (a.dtype == FLUX_CUDA_F32 ? 4 : 2));
   P.gate = a.gate;

@@ -118,6 +118,11 @@ def test_product_with_every_size_of_scale(fx, ctx, fmt, ex, ew, sx, sw, M, N, K)
     (32, -50, -50, 2.0 ** 50, 2.0 ** 50, 40),    # or is beyond f32
     (32, -60, -60, 2.0 ** 100, 2.0 ** 100, -70),
     (32, 50, 50, 2.0 ** -100, 2.0 ** -100, 70),
+    (16, 0, 0, 2.0 ** 60, 2.0 ** 60, -60),        # the scales alone take the sum out of f32
+    (16, 0, 0, 2.0 ** 90, 1.3 * 2.0 ** 90, -149 + 23),
+    (32, 50, 50, 2.0 ** -127, 2.0 ** -127, 100),
+    (32, 50, 50, 1.7 * 2.0 ** -140, 2.0 ** -120, 120),
+    (32, -60, -60, 2.0 ** 120, 2.0 ** 120, -30),
     (16, 0, 0, 0.5, 1.7, 0)])
 def test_gated_product_with_every_size_of_scale(fx, ctx, fmt, ex, ew, sx, sw, eg, in_place, M, N, K):
     """gate and residual: one rounding more, and that of the sum with the residual. A gate of 0 leaves the residual."""
