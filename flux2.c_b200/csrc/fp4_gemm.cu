@@ -192,10 +192,10 @@ __device__ __forceinline__ void fp4_emit(const uint32_t (&r)[16], float (&v)[16]
 template <int DT, int SP, int R, bool STEPS>
 __device__ __forceinline__ void fp4_join(uint32_t part, int splits, int m, int m_end, int n, int N, uint8_t *out,
                                          long long pitch, const uint8_t *res, long long res_pitch,
-                                         const Fp4GemmParams &P, float &mx) {
+                                         const Fp4GemmParams &P, const Fp4Factor (&early)[4], float &mx) {
   Fp4Factor f[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = fp4_column<STEPS>(P, n + i < N ? n + i : N - 1);
+  for (int i = 0; i < 4; ++i) f[i] = STEPS ? early[i] : fp4_column<STEPS>(P, n + i < N ? n + i : N - 1);
   for (; m < m_end; m += 4 * R) {
     float4 v[SP][R];
     float y[R][4];  // the residual, all of it requested before anything is stored (it may be `out`)
@@ -347,6 +347,12 @@ __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const
     const int nl = q * 32 + lane, n = n0 + nl;
     const int live = P.M - m0 < BM ? P.M - m0 : BM;
     const Fp4Factor f = fp4_column<STEPS>(P, n < P.N ? n : P.N - 1);
+    Fp4Factor f4[4];  // of the columns that this lane joins; worked out behind the products where that takes a while
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = n0 + lane * 4 + i;
+      if (STEPS) f4[i] = P.splits > 1 ? fp4_column<STEPS>(P, c < P.N ? c : P.N - 1) : f;
+    }
     float mx = 0.f;
     const long long pitch = P.pitch, res_pitch = P.res_pitch;
     uint8_t *out = static_cast<uint8_t *>(P.out) + m0 * pitch + n * static_cast<long long>(FP4_SIZE<DT>);
@@ -390,9 +396,9 @@ __global__ void __launch_bounds__(F_THREADS, DEEP ? 1 : 2) gemm_fp4_kernel(const
         const uint32_t mine = smem_u32(part) + lane * 16;
         uint8_t *o = static_cast<uint8_t *>(P.out) + m0 * pitch + nj * static_cast<long long>(FP4_SIZE<DT>);
         const uint8_t *r = P.residual ? reinterpret_cast<const uint8_t *>(P.residual) + m0 * res_pitch + nj * 4LL : nullptr;
-        if (P.splits <= 2) fp4_join<DT, 2, 8, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, mx);
-        else if (P.splits <= 4) fp4_join<DT, 4, 4, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, mx);
-        else fp4_join<DT, 8, 2, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, mx);
+        if (P.splits <= 2) fp4_join<DT, 2, 8, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, f4, mx);
+        else if (P.splits <= 4) fp4_join<DT, 4, 4, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, f4, mx);
+        else fp4_join<DT, 8, 2, STEPS>(mine, P.splits, first, end, nj, P.N, o, pitch, r, res_pitch, P, f4, mx);
       }
     }
     sat_report(P.err + 1, DT == FLUX_CUDA_F16, mx);
